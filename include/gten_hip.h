@@ -181,6 +181,142 @@ const char* nc_debug_ew_route(int silu, int dtype, int rows, int cols);
 /* Greedy pick of greedy_sample (src/gten/sampler.cpp:33-41): first index of
  * the maximum. */
 int nc_argmax(const float* x, int n, int32_t* out, void* stream);
+/* ---- serving many requests at once: paged K/V and adapters --------------------
+ * No counterpart in the reference, which runs one sequence.  Each step of a
+ * server has some new rows of each of n_req requests, one request's rows
+ * after the other's, and keeps all K/V rows in pages of page_size positions
+ * of a common cache.  nc_paged_plan builds the step's tables on the device
+ * from the requests' lengths; nc_lora_add, nc_paged_append and nc_paged_attn
+ * stand where nc_bias_add, nc_rotary_emb and nc_qkv_attn stand for one
+ * sequence; nc_paged_commit ends the step.  The lengths stay on the device,
+ * so a step can be captured into a HIP graph and replayed: no call below
+ * allocates, synchronizes or reads device memory on the host, and none keeps
+ * state between calls.  Arrays are device memory unless said otherwise.
+ * Activation rows here start at 16-byte addresses (data and pitch). */
+#define NC_PAGED_MAX_REQ 4096
+#define NC_PAGED_MAX_KV (1 << 24) /* positions of one request */
+
+/* The cache of one layer: values [n_pages][n_kv_heads][page_size][d_head] of
+ * fp16 (dtype NC_F16) or int8 codes (NC_Q8) with one fp16 delta per 32 of
+ * them, [n_pages][n_kv_heads][page_size][d_head / 32] (nc_paged_cache_bytes;
+ * 16-byte aligned).  page_size: a power of two from 16 to 1024; d_head: 64 or
+ * 128.  Position p of a request is row p % page_size of page
+ * block_table[request][p / page_size]; its slot is page * page_size + that
+ * row.  Attention reads the values as fp16, so a Q8 cache holds values within
+ * fp16's range. */
+typedef struct nc_paged_cache {
+    void* k;
+    void* v;
+    void* k_deltas; /* NC_Q8 only */
+    void* v_deltas;
+    int dtype;
+    int n_pages;
+    int page_size;
+    int n_kv_heads;
+    int d_head;
+} nc_paged_cache;
+
+/* Which pages are free: a stack of page ids, the top at state[0] - 1.
+ * state[0] = free pages, state[1] = free pages once the plan is committed,
+ * state[2] = the plan's status (0, or the sum of what stopped it:
+ * NC_PLAN_*), state[3] unused. */
+typedef struct nc_page_pool {
+    int32_t* free_pages; /* [n_pages] */
+    int32_t* state;      /* [4] */
+    int n_pages;
+    int page_size;
+} nc_page_pool;
+#define NC_PLAN_NO_PAGES 1 /* the free pages do not suffice */
+#define NC_PLAN_TOO_LONG 2 /* a request passes max_kv or its block table */
+#define NC_PLAN_NO_ROWS 4  /* more rows than max_tokens */
+#define NC_PLAN_BAD_LEN 8  /* a length is negative or above max_new */
+
+/* One step's requests.  max_new and max_kv are the host's upper bounds of a
+ * request's new rows and of its positions with them (a looser bound costs
+ * time, never correctness). */
+typedef struct nc_paged_batch {
+    int n_req;      /* up to NC_PAGED_MAX_REQ */
+    int max_tokens; /* rows of the step's tensors, requests' rows first */
+    int max_pages;  /* width of block_table */
+    int max_new;
+    int max_kv;
+    const int32_t* new_len; /* [n_req] new rows of each request, 0 for an idle one */
+    int32_t* seq_len;       /* [n_req] positions already cached */
+    int32_t* block_table;   /* [n_req][max_pages] page ids */
+    int32_t* row_start;     /* [n_req + 1] plan: the requests' first rows, then the rows' count */
+    int32_t* kv_len;        /* [n_req] plan: seq_len + new_len */
+    int32_t* positions;     /* [max_tokens] plan: each row's position, -1 behind the last */
+    int32_t* slots;         /* [max_tokens] plan: each row's cache slot, -1 behind the last */
+} nc_paged_batch;
+
+/* Bytes of k (and v) and of k_deltas (and v_deltas) of a cache; on the host. */
+int nc_paged_cache_bytes(int dtype, int n_pages, int page_size, int n_kv_heads, int d_head, size_t* code_bytes,
+                         size_t* delta_bytes);
+/* All pages free, in ascending order from the top of the stack. */
+int nc_page_pool_init(const nc_page_pool* pool, void* stream);
+/* The step's tables from the requests' lengths: row_start, kv_len, positions,
+ * slots, and in block_table the pages of the new positions, taken from the
+ * pool's stack in the order of requests and positions.  It may be run again
+ * before the commit, with other lengths too: what it reads it leaves as it
+ * was.  A plan that cannot be met sets state[2] and plans no rows
+ * (row_start all 0, positions and slots -1, kv_len = seq_len, no pages
+ * taken), so that the calls after it do nothing. */
+int nc_paged_plan(const nc_page_pool* pool, const nc_paged_batch* batch, void* stream);
+/* Ends the step: seq_len = kv_len, and the planned pages leave the pool.
+ * Requests with finished[r] != 0 (NULL: none) get length 0 and their pages go
+ * back to the pool.  Entries that are no page are passed over. */
+int nc_paged_commit(const nc_page_pool* pool, const nc_paged_batch* batch, const int32_t* finished, void* stream);
+/* Rotates the q and k rows at batch->positions (nc_rotary_emb's values, with
+ * nc_rope_table's pairs [rope_rows][d_half]; rope = NULL: no rotation), and
+ * stores q to q_out and k and v to the cache at batch->slots.  q, k and v:
+ * [max_tokens] rows of one activation dtype; q_out: NC_F16 or NC_Q8, and q
+ * itself if of its dtype; q and q_out may both be NULL.  Rows whose slot lies
+ * outside the cache or whose position lies outside the rope table are passed
+ * over. */
+int nc_paged_append(const nc_tensor* q, const nc_tensor* k, const nc_tensor* v, nc_tensor* q_out,
+                    const nc_paged_cache* cache, const nc_paged_batch* batch, const float* rope, int rope_rows,
+                    int d_half, void* stream);
+/* Causal attention of each request's new rows, the last of its kv_len
+ * positions, over its pages (the new rows' own k and v appended before):
+ * out = softmax(q . k / sqrt(d_head)) v, n_heads a multiple of the cache's
+ * n_kv_heads.  window > 0: a row at position p sees positions above
+ * p - window and those below n_sink; 0: all up to its own.  Only pages that
+ * hold a visible position are read; positions on an entry that is no page are
+ * not seen, and a row that sees nothing is 0.  What lies in unseen positions
+ * (NaN too) has no effect.  q and out: rows of NC_F16 or NC_Q8.  Unlike
+ * nc_qkv_attn it is not bit for bit the reference's: products on the matrix
+ * cores with fp16 factors, statistics and sums in fp32, summed in an order
+ * that depends on sizes and lengths alone.  workspace: at least
+ * nc_paged_attn_workspace's bytes of device memory (16-byte aligned), which
+ * calls that may overlap must not share; its contents need no preparation. */
+int nc_paged_attn(const nc_tensor* q, const nc_paged_cache* cache, const nc_paged_batch* batch, nc_tensor* out,
+                  int n_heads, int window, int n_sink, void* workspace, size_t workspace_bytes, void* stream);
+/* On the host: depends on the sizes alone, never on the arrays' contents. */
+int nc_paged_attn_workspace(const nc_paged_cache* cache, const nc_paged_batch* batch, int n_heads, int window,
+                            int n_sink, size_t* bytes);
+
+/* Low-rank adapters of one projection [n, k]: fp16 a [n_adapters][rank][k]
+ * and b [n_adapters][n][rank] (16-byte aligned), fp32 scale [n_adapters];
+ * rank up to NC_LORA_MAX_RANK (smaller ones padded with zeros), k a multiple
+ * of 32. */
+#define NC_LORA_MAX_RANK 128
+typedef struct nc_lora {
+    const uint16_t* a;
+    const uint16_t* b;
+    const float* scale;
+    int n_adapters;
+    int rank;
+    int k;
+    int n;
+} nc_lora;
+/* out = base + scale (x a^T) b^T for each request's rows, with its adapter
+ * (adapter[r], [n_req]; one that is no adapter, as -1: out = base).  x: rows
+ * of NC_F16 or NC_Q8, k wide; base: fp32 rows, n wide, as nc_matmul_2d leaves
+ * them with an fp32 output; out: NC_F32 (base itself too), NC_F16 or NC_Q8.
+ * Requests' rows are [row_start[r], row_start[r + 1]), at most max_new each
+ * (further ones are left as they were).  Sums in fp32. */
+int nc_lora_add(const nc_tensor* x, const nc_tensor* base, const nc_lora* lora, const int32_t* adapter,
+                const int32_t* row_start, int n_req, int max_new, nc_tensor* out, void* stream);
 /* ---- tokenizers (host) ----------------------------------------------------
  * The reference's LLamaTokenizer (src/gten/tokenizer.cpp:25-248: BPE with
  * scores, byte fallback) and Gpt2Tokenizer (tokenizer.cpp:251-334: regex

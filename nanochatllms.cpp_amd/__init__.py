@@ -43,6 +43,35 @@ class ModelConfig(C.Structure):
                 ("n_kv_heads", C.c_int * MAX_LAYERS), ("n_ffn", C.c_int * MAX_LAYERS)]
 
 
+class PagedCache(C.Structure):
+    """nc_paged_cache: one layer's K/V pages (no ownership)."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_deltas", C.c_void_p), ("v_deltas", C.c_void_p),
+                ("dtype", C.c_int), ("n_pages", C.c_int), ("page_size", C.c_int), ("n_kv_heads", C.c_int),
+                ("d_head", C.c_int)]
+
+
+class PagePool(C.Structure):
+    """nc_page_pool: the stack of free pages and its counters."""
+    _fields_ = [("free_pages", C.c_void_p), ("state", C.c_void_p), ("n_pages", C.c_int), ("page_size", C.c_int)]
+
+
+class PagedBatch(C.Structure):
+    """nc_paged_batch: one step's requests and their tables."""
+    _fields_ = [("n_req", C.c_int), ("max_tokens", C.c_int), ("max_pages", C.c_int), ("max_new", C.c_int),
+                ("max_kv", C.c_int), ("new_len", C.c_void_p), ("seq_len", C.c_void_p), ("block_table", C.c_void_p),
+                ("row_start", C.c_void_p), ("kv_len", C.c_void_p), ("positions", C.c_void_p), ("slots", C.c_void_p)]
+
+
+class Lora(C.Structure):
+    """nc_lora: the low-rank adapters of one projection."""
+    _fields_ = [("a", C.c_void_p), ("b", C.c_void_p), ("scale", C.c_void_p), ("n_adapters", C.c_int),
+                ("rank", C.c_int), ("k", C.c_int), ("n", C.c_int)]
+
+
+PLAN_NO_PAGES, PLAN_TOO_LONG, PLAN_NO_ROWS, PLAN_BAD_LEN = 1, 2, 4, 8  # nc_page_pool's state[2]
+PAGED_MAX_REQ, LORA_MAX_RANK = 4096, 128
+
+
 def make_config(arch, wdtype, n_vocab, n_embd, n_layers, n_heads, n_kv_heads, n_ffn, max_ctx, eos=-1,
                 rope_pct=1.0, d_head=64, cls=ModelConfig):
     c = cls()
@@ -138,6 +167,7 @@ def lib():
     L = C.CDLL(LIB_PATH)
     VP, I, F, SZ, U64 = C.c_void_p, C.c_int, C.c_float, C.c_size_t, C.c_uint64
     TP = C.POINTER(Tensor)
+    CP, PP, BP = C.POINTER(PagedCache), C.POINTER(PagePool), C.POINTER(PagedBatch)
     sig = {
         "nc_init": (I, [I]), "nc_last_error": (C.c_char_p, []), "nc_malloc": (I, [C.POINTER(VP), SZ]),
         "nc_free": (I, [VP]), "nc_memcpy_h2d": (I, [VP, VP, SZ]), "nc_memcpy_d2h": (I, [VP, VP, SZ]),
@@ -185,6 +215,13 @@ def lib():
         "nc_model_sample_begin": (I, [VP, VP, I, F, I, C.c_uint32]),
         "nc_model_sample_steps": (I, [VP, I, VP]),
         "nc_model_get_config": (I, [VP, C.POINTER(ModelConfig)]),
+        "nc_paged_cache_bytes": (I, [I, I, I, I, I, C.POINTER(SZ), C.POINTER(SZ)]),
+        "nc_page_pool_init": (I, [PP, VP]), "nc_paged_plan": (I, [PP, BP, VP]),
+        "nc_paged_commit": (I, [PP, BP, VP, VP]),
+        "nc_paged_append": (I, [TP, TP, TP, TP, CP, BP, VP, I, I, VP]),
+        "nc_paged_attn": (I, [TP, CP, BP, TP, I, I, I, VP, SZ, VP]),
+        "nc_paged_attn_workspace": (I, [CP, BP, I, I, I, C.POINTER(SZ)]),
+        "nc_lora_add": (I, [TP, TP, C.POINTER(Lora), VP, VP, I, I, TP, VP]),
         "nc_greedy_sample": (I, [VP, VP, C.c_char_p, I, TEXT_SINK, VP, C.POINTER(I)]),
         "nc_topk_sample": (I, [VP, VP, C.c_char_p, I, F, I, C.c_uint32, TEXT_SINK, VP, C.POINTER(I)]),
     }

@@ -1,0 +1,68 @@
+// nc_paged.h -- what the kernels of batched serving share: argument checks
+// and the places of requests' rows.
+#pragma once
+
+#include "nc_device.h"
+#include "nc_runtime.h"
+
+namespace nc {
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Activation rows as these kernels take them: 16-byte aligned, whole rows.
+inline bool paged_rows_ok(const nc_tensor* t, int rows, int cols)
+{
+    return t && t->data && is_act(t->dtype) && t->rows >= rows && t->cols == cols && aligned16(t->data) &&
+           t->pitch >= act_pitch(t->dtype, cols) && (t->pitch & 15) == 0;
+}
+
+int check_cache(const char* what, const nc_paged_cache* c);
+int check_batch(const char* what, const nc_paged_batch* b, int page_size);
+
+// Rows [first, first + n) of request r, clamped to the step's rows so that no
+// table, however wrong, leads outside the tensors.
+struct RowSpan {
+    int first, n;
+};
+__device__ __forceinline__ RowSpan request_rows(const int* row_start, int r, int max_tokens, int max_new)
+{
+    const int a = min(max(row_start[r], 0), max_tokens);
+    const int b = min(max(row_start[r + 1], 0), max_tokens);
+    return {a, min(max(b - a, 0), max_new)};
+}
+
+// Work is cut into tiles of `m` units, a request's row holding `per_row`
+// units, with no tile across two requests.  The tiles of request r are
+// numbered from first_tile(r) = floor(row_start[r] per_row / m) + r: floors
+// and one more per request leave each request at least the
+// ceil(rows per_row / m) numbers it needs, and tile_slots() numbers hold them
+// all, so a launch needs no table of tiles and no lengths on the host.
+__device__ __forceinline__ int first_tile(int start, int r, int per_row, int m, int max_tokens)
+{
+    const int s = min(max(start, 0), max_tokens);
+    return (int)((long long)s * per_row / m) + r;
+}
+inline long long tile_slots(int max_tokens, int n_req, int per_row, int m)
+{
+    return (long long)max_tokens * per_row / m + n_req;
+}
+
+// The request of tile number t: the last one whose first tile is at most t,
+// found by a wavefront that probes 64 requests at a time.
+__device__ __forceinline__ int tile_request(const int* row_start, int n_req, int t, int per_row, int m, int max_tokens)
+{
+    const int lane = threadIdx.x & (kWave - 1);
+    int lo = 0, len = n_req;
+    while (true) {
+        const int step = (len + kWave - 1) / kWave;
+        const int r = lo + lane * step;
+        const bool at = lane * step < len && first_tile(row_start[min(r, n_req - 1)], r, per_row, m, max_tokens) <= t;
+        const int c = __popcll(__ballot(at));
+        if (c == 0) return lo;  // tables that are no row starts
+        lo += (c - 1) * step;
+        len = min(step, n_req - lo);
+        if (step == 1) return __builtin_amdgcn_readfirstlane(lo);
+    }
+}
+
+}  // namespace nc

@@ -1,0 +1,497 @@
+// nc_paged.hip -- the bookkeeping of batched serving: the step's tables, the
+// page pool, and new K/V rows into the pages.
+#include "nc_act.h"
+#include "nc_paged.h"
+
+namespace nc {
+
+int check_cache(const char* what, const nc_paged_cache* c)
+{
+    NC_CHECK_ARG(c && c->k && c->v, "%s: null cache", what);
+    NC_CHECK_ARG(c->dtype == NC_F16 || c->dtype == NC_Q8, "%s: cache dtype %d (F16 or Q8)", what, c->dtype);
+    NC_CHECK_ARG(c->d_head == 64 || c->d_head == 128, "%s: head size %d (64 or 128)", what, c->d_head);
+    NC_CHECK_ARG(c->page_size >= 16 && c->page_size <= 1024 && (c->page_size & (c->page_size - 1)) == 0,
+                 "%s: page size %d (a power of two from 16 to 1024)", what, c->page_size);
+    NC_CHECK_ARG(c->n_kv_heads >= 1 && c->n_kv_heads <= 1024, "%s: %d kv heads", what, c->n_kv_heads);
+    NC_CHECK_ARG(c->n_pages >= 1 && (long long)c->n_pages * c->page_size <= 0x7FFFFFFFll,
+                 "%s: %d pages of %d positions (slots are 32 bits)", what, c->n_pages, c->page_size);
+    NC_CHECK_ARG(aligned16(c->k) && aligned16(c->v), "%s: cache addresses are not 16-byte aligned", what);
+    if (c->dtype == NC_Q8)
+        NC_CHECK_ARG(c->k_deltas && c->v_deltas && aligned16(c->k_deltas) && aligned16(c->v_deltas),
+                     "%s: a Q8 cache needs 16-byte aligned deltas", what);
+    return NC_OK;
+}
+
+int check_batch(const char* what, const nc_paged_batch* b, int page_size)
+{
+    NC_CHECK_ARG(b, "%s: null batch", what);
+    NC_CHECK_ARG(b->n_req >= 1 && b->n_req <= NC_PAGED_MAX_REQ, "%s: %d requests (1 to %d)", what, b->n_req,
+                 NC_PAGED_MAX_REQ);
+    NC_CHECK_ARG(b->max_tokens >= 0 && b->max_tokens <= (1 << 26), "%s: %d rows", what, b->max_tokens);
+    NC_CHECK_ARG(b->max_new >= 0 && b->max_kv >= 0 && b->max_kv <= NC_PAGED_MAX_KV, "%s: bounds max_new %d, max_kv %d",
+                 what, b->max_new, b->max_kv);
+    NC_CHECK_ARG(b->max_pages >= 1 && (long long)b->max_pages * page_size >= b->max_kv &&
+                     (long long)b->max_pages * b->n_req <= 0x7FFFFFFFll,
+                 "%s: %d pages a request do not hold max_kv %d positions", what, b->max_pages, b->max_kv);
+    NC_CHECK_ARG(b->row_start && b->kv_len && b->block_table && b->positions && b->slots, "%s: null table", what);
+    return NC_OK;
+}
+
+// ------------------------------------------------------------------- plan --
+
+constexpr int kPlanThreads = 256;
+constexpr int kPlanRows = 1024;  // rows of one workgroup
+constexpr int kPlanMaxPer = NC_PAGED_MAX_REQ / kPlanThreads;
+
+// Sum of v over the workgroup's threads before this one; *total = over all.
+template <typename T, int THREADS>
+__device__ __forceinline__ T block_scan(T v, T* tmp, T* total)
+{
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    T s = v;
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) {
+        const T o = __shfl_up(s, d);
+        if (lane >= d) s += o;
+    }
+    __syncthreads();
+    if (lane == kWave - 1) tmp[wave] = s;
+    __syncthreads();
+    T before = 0, sum = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / kWave; w++) {
+        if (w < wave) before += tmp[w];
+        sum += tmp[w];
+    }
+    *total = sum;
+    return before + s - v;
+}
+
+// One launch, no order between workgroups: each scans all requests' lengths
+// itself (two exclusive sums, of rows and of new pages) and then writes its
+// share of the rows' positions and slots.  The scan reads 8 bytes a request
+// from L2; a second launch would cost more than all of them do.  Nothing
+// that is read is written: new table entries lie behind the entries that the
+// requests have, and each is written by the row that opens the page, the
+// row whose position is a multiple of the page size.
+__global__ __launch_bounds__(kPlanThreads) void k_paged_plan(nc_paged_batch b, const int* __restrict__ free_pages,
+                                                             int* __restrict__ state, int n_pages, int lps)
+{
+    __shared__ int row0[NC_PAGED_MAX_REQ + 1];
+    __shared__ int page0[NC_PAGED_MAX_REQ];
+    __shared__ long long tmp64[kPlanThreads / kWave];
+    __shared__ int status_sh;
+    const int tid = threadIdx.x, ps = 1 << lps;
+    const int per = (b.n_req + kPlanThreads - 1) / kPlanThreads;
+    const int r0 = tid * per;
+    if (tid == 0) status_sh = 0;
+
+    long long rows = 0, pages = 0;
+    int status = 0;
+#pragma unroll 1
+    for (int i = 0; i < per; i++) {
+        const int r = r0 + i;
+        if (r >= b.n_req) break;
+        const int n = b.new_len[r], s = b.seq_len[r];
+        if (n < 0 || n > b.max_new || s < 0) status |= NC_PLAN_BAD_LEN;
+        const long long kv = (long long)s + n;
+        if (kv > b.max_kv) status |= NC_PLAN_TOO_LONG;
+        rows += n;
+        pages += ((kv + ps - 1) >> lps) - (((long long)s + ps - 1) >> lps);
+    }
+    long long n_rows, n_new;
+    long long row = block_scan<long long, kPlanThreads>(rows, tmp64, &n_rows);
+    long long page = block_scan<long long, kPlanThreads>(pages, tmp64, &n_new);
+    const int n_free = min(max(state[0], 0), n_pages);
+    if (n_rows > b.max_tokens) status |= NC_PLAN_NO_ROWS;
+    if (n_new > n_free) status |= NC_PLAN_NO_PAGES;
+    if (status) atomicOr(&status_sh, status);
+    __syncthreads();
+    status = status_sh;
+    const bool ok = status == 0, first = blockIdx.x == 0;
+
+#pragma unroll 1
+    for (int i = 0; i < per; i++) {
+        const int r = r0 + i;
+        if (r >= b.n_req) break;
+        const int n = b.new_len[r], s = b.seq_len[r];
+        row0[r] = (int)row;
+        page0[r] = (int)page;
+        if (first) {
+            b.row_start[r] = ok ? (int)row : 0;
+            b.kv_len[r] = ok ? s + n : s;
+        }
+        row += n;
+        page += (((long long)s + n + ps - 1) >> lps) - (((long long)s + ps - 1) >> lps);
+    }
+    if (first && tid == 0) {
+        b.row_start[b.n_req] = ok ? (int)n_rows : 0;
+        state[1] = ok ? n_free - (int)n_new : state[0];
+        state[2] = status;
+    }
+    __syncthreads();
+
+    const int end = min((int)(blockIdx.x + 1) * kPlanRows, b.max_tokens);
+    for (int t = blockIdx.x * kPlanRows + tid; t < end; t += kPlanThreads) {
+        int pos = -1, slot = -1;
+        if (ok && t < (int)n_rows) {
+            // the last request whose first row is at most t: it has a row t
+            int lo = 0, hi = b.n_req;
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (row0[mid] <= t) lo = mid;
+                else hi = mid;
+            }
+            const int s = b.seq_len[lo];
+            pos = s + t - row0[lo];
+            const int pi = pos >> lps, have = (int)(((long long)s + ps - 1) >> lps);
+            int id;
+            if (pi < have) {
+                id = b.block_table[(size_t)lo * b.max_pages + pi];
+            } else {
+                id = free_pages[n_free - 1 - (page0[lo] + pi - have)];
+                if ((pos & (ps - 1)) == 0) b.block_table[(size_t)lo * b.max_pages + pi] = id;
+            }
+            if ((unsigned)id < (unsigned)n_pages) slot = id * ps + (pos & (ps - 1));
+        }
+        b.positions[t] = pos;
+        b.slots[t] = slot;
+    }
+}
+
+constexpr int kCommitThreads = 1024;
+
+// One workgroup: a page's place on the stack depends on every request before
+// it.  Released pages are counted per request (a wavefront a request), the
+// counts summed, and then stored in the order of requests and positions.
+__global__ __launch_bounds__(kCommitThreads) void k_paged_commit(nc_paged_batch b, int* __restrict__ free_pages,
+                                                                 int* __restrict__ state, int n_pages, int lps,
+                                                                 const int* __restrict__ finished)
+{
+    __shared__ int count[NC_PAGED_MAX_REQ];
+    __shared__ int tmp[kCommitThreads / kWave];
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+    constexpr int kWaves = kCommitThreads / kWave;
+    const int n_free = min(max(state[1], 0), n_pages);
+    auto held = [&](int r) {  // pages of request r, within its table
+        const long long n = ((long long)max(b.kv_len[r], 0) + (1 << lps) - 1) >> lps;
+        return (int)(n < b.max_pages ? n : b.max_pages);
+    };
+    if (finished) {
+        for (int r = wave; r < b.n_req; r += kWaves) {
+            int c = 0;
+            if (finished[r]) {
+                const int n = held(r);
+                for (int p = lane; p < n; p += kWave)
+                    c += (unsigned)b.block_table[(size_t)r * b.max_pages + p] < (unsigned)n_pages;
+#pragma unroll
+                for (int d = kWave / 2; d; d >>= 1) c += __shfl_xor(c, d);
+            }
+            if (lane == 0) count[r] = c;
+        }
+        __syncthreads();
+        const int per = (b.n_req + kCommitThreads - 1) / kCommitThreads, r0 = tid * per;
+        int sum = 0, total;
+        for (int i = 0; i < per && r0 + i < b.n_req; i++) sum += count[r0 + i];
+        int at = block_scan<int, kCommitThreads>(sum, tmp, &total);
+        for (int i = 0; i < per && r0 + i < b.n_req; i++) {
+            const int c = count[r0 + i];
+            count[r0 + i] = at;
+            at += c;
+        }
+        __syncthreads();
+        for (int r = wave; r < b.n_req; r += kWaves) {
+            if (!finished[r]) continue;
+            int dst = n_free + count[r];
+            const int n = held(r);
+            for (int p0 = 0; p0 < n; p0 += kWave) {
+                const int p = p0 + lane;
+                int* entry = b.block_table + (size_t)r * b.max_pages + p;
+                const int id = p < n ? *entry : -1;
+                const bool is_page = (unsigned)id < (unsigned)n_pages;
+                const unsigned long long m = __ballot(is_page);
+                const int to = dst + __popcll(m & ((1ull << lane) - 1));
+                if (is_page && to < n_pages) free_pages[to] = id;
+                if (p < n) *entry = -1;
+                dst += __popcll(m);
+            }
+        }
+        __syncthreads();  // kv_len is read above and written below
+        if (tid == 0) state[0] = state[1] = min(n_free + total, n_pages);
+    } else if (tid == 0) {
+        state[0] = n_free;
+    }
+    for (int r = tid; r < b.n_req; r += kCommitThreads) {
+        const int kv = finished && finished[r] ? 0 : b.kv_len[r];
+        b.seq_len[r] = kv;
+        b.kv_len[r] = kv;
+    }
+}
+
+__global__ __launch_bounds__(256) void k_pool_init(int* __restrict__ free_pages, int* __restrict__ state, int n_pages)
+{
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i < n_pages) free_pages[i] = n_pages - 1 - i;
+    if (i < 4) state[i] = i < 2 ? n_pages : 0;
+}
+
+// ----------------------------------------------------------------- append --
+
+struct AppendArgs {
+    const uint8_t *q, *k, *v;
+    uint8_t* q_out;
+    int q_pitch, k_pitch, v_pitch, o_pitch;
+    uint8_t *kc, *vc;
+    uint16_t *kd, *vd;
+    const int *positions, *slots;
+    const float2* rope;
+    int rope_rows, d_half;
+    int rows, hq, hkv, n_slots, lps;
+};
+
+// rope8 for any d_half: the partner of value e sits in register e' % 8 of
+// lane e' / 8 of the head.
+__device__ __forceinline__ void rope8_any(float (&x)[8], int l, int d_half, const float2* cs)
+{
+    const int lane = threadIdx.x & (kWave - 1), head = lane - l;
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const int e = 8 * l + i;
+        const bool lo = e < d_half, in = e < 2 * d_half;
+        const int pe = lo ? e + d_half : (in ? e - d_half : e);
+        float xp = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const float s = __shfl(x[j], head + (pe >> 3));
+            if ((pe & 7) == j) xp = s;
+        }
+        y[i] = x[i];
+        if (in) {
+            const float2 c = cs[lo ? e : e - d_half];
+            y[i] = lo ? x[i] * c.x - xp * c.y : xp * c.y + x[i] * c.x;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = y[i];
+}
+
+// Eight values per thread over every (row, chunk of q | k | v), as k_rope8:
+// a head's 8 or 16 threads sit side by side in a wavefront, the values that a
+// rotation pairs are d_half / 8 lanes apart, and a Q8 block is a quad.  Each
+// value is read and written once, bound by that traffic.  The roundings are
+// the activation rows' own (q8_quantize, fp16 nearest even), so the cache
+// holds what nc_rotary_emb would have stored.
+template <int ADT, int QDT, int CDT, int D>
+__global__ __launch_bounds__(256) void k_paged_append(AppendArgs a)
+{
+    constexpr int kL = D / 8;  // threads of a head
+    const int nh = a.hq + 2 * a.hkv, nc8 = nh * kL;
+    const long long t = (long long)blockIdx.x * 256 + threadIdx.x;
+    const int r = (int)(t / nc8), c = (int)(t - (long long)r * nc8);
+    if (r >= a.rows) return;  // whole heads, as the returns below
+    const int slot = a.slots[r];
+    if ((unsigned)slot >= (unsigned)a.n_slots) return;
+    const int pos = a.positions[r];
+    if (a.rope && (unsigned)pos >= (unsigned)a.rope_rows) return;
+    int h = c / kL;
+    const int l = c % kL;
+    const int kind = h < a.hq ? 0 : (h < a.hq + a.hkv ? 1 : 2);
+    h -= kind == 0 ? 0 : (kind == 1 ? a.hq : a.hq + a.hkv);
+    const int heads = kind == 0 ? a.hq : a.hkv;
+    const uint8_t* in = kind == 0 ? a.q + (size_t)r * a.q_pitch
+                                  : (kind == 1 ? a.k + (size_t)r * a.k_pitch : a.v + (size_t)r * a.v_pitch);
+    float x[8];
+    act_load8<ADT>(in, h * kL + l, heads * D, x);
+    if (a.rope && kind < 2) {
+        const float2* cs = a.rope + (size_t)pos * a.d_half;
+        if ((a.d_half & 7) == 0) {
+            const int nl = a.d_half >> 3;
+            const bool lo = l < nl, turned = l < 2 * nl;
+            const int lane = threadIdx.x & (kWave - 1);
+            const int partner = lo ? lane + nl : (turned ? lane - nl : lane);
+            float xp[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) xp[i] = __shfl(x[i], partner);
+            if (turned) {
+                const float2* p = cs + (lo ? l : l - nl) * 8;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float2 w = p[i];
+                    x[i] = lo ? x[i] * w.x - xp[i] * w.y : xp[i] * w.y + x[i] * w.x;
+                }
+            }
+        } else {
+            rope8_any(x, l, a.d_half, cs);
+        }
+    }
+    if (kind == 0) {
+        act_store8<QDT>(a.q_out + (size_t)r * a.o_pitch, h * kL + l, heads * D, x);
+        return;
+    }
+    const size_t row = ((((size_t)(slot >> a.lps) * a.hkv + h) << a.lps) + (slot & ((1 << a.lps) - 1)));
+    uint8_t* out = (kind == 1 ? a.kc : a.vc) + row * (CDT == Q8 ? D : 2 * D);
+    if (CDT == Q8) {
+        // act_store8's Q8 row with its deltas in an array of their own
+        int8_t q[8];
+        uint16_t d16;
+        q8_quant8(x, q, &d16);
+        uint32_t w[2] = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 8; i++) w[i >> 2] |= (uint32_t)(uint8_t)q[i] << (8 * (i & 3));
+        reinterpret_cast<uint2*>(out)[l] = make_uint2(w[0], w[1]);
+        if ((l & 3) == 0) (kind == 1 ? a.kd : a.vd)[row * (D / 32) + (l >> 2)] = d16;
+    } else {
+        act_store8<F16>(out, l, 0, x);
+    }
+}
+
+template <int ADT, int QDT, int CDT>
+static void append_launch(const AppendArgs& a, int d, unsigned grid, hipStream_t st)
+{
+    if (d == 64) hipLaunchKernelGGL((k_paged_append<ADT, QDT, CDT, 64>), dim3(grid), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_paged_append<ADT, QDT, CDT, 128>), dim3(grid), dim3(256), 0, st, a);
+}
+template <int ADT>
+static void append_launch(const AppendArgs& a, int qdt, int cdt, int d, unsigned grid, hipStream_t st)
+{
+    if (qdt == Q8) cdt == Q8 ? append_launch<ADT, Q8, Q8>(a, d, grid, st) : append_launch<ADT, Q8, F16>(a, d, grid, st);
+    else cdt == Q8 ? append_launch<ADT, F16, Q8>(a, d, grid, st) : append_launch<ADT, F16, F16>(a, d, grid, st);
+}
+
+static int log2_of(int v) { return __builtin_ctz((unsigned)v); }
+
+static int check_pool(const char* what, const nc_page_pool* p)
+{
+    NC_CHECK_ARG(p && p->free_pages && p->state, "%s: null pool", what);
+    NC_CHECK_ARG(p->page_size >= 16 && p->page_size <= 1024 && (p->page_size & (p->page_size - 1)) == 0,
+                 "%s: page size %d (a power of two from 16 to 1024)", what, p->page_size);
+    NC_CHECK_ARG(p->n_pages >= 1 && (long long)p->n_pages * p->page_size <= 0x7FFFFFFFll,
+                 "%s: %d pages of %d positions (slots are 32 bits)", what, p->n_pages, p->page_size);
+    return NC_OK;
+}
+
+static bool overlap(const void* a, size_t an, const void* b, size_t bn)
+{
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y + bn && y < x + an;
+}
+
+}  // namespace nc
+
+using namespace nc;
+
+extern "C" {
+
+int nc_paged_cache_bytes(int dtype, int n_pages, int page_size, int n_kv_heads, int d_head, size_t* code_bytes,
+                         size_t* delta_bytes)
+{
+    NC_CHECK_ARG(code_bytes && delta_bytes, "paged_cache_bytes: null result");
+    alignas(16) static char any[16];
+    const nc_paged_cache c{any, any, any, any, dtype, n_pages, page_size, n_kv_heads, d_head};
+    if (int s = check_cache("paged_cache_bytes", &c)) return s;
+    const size_t values = (size_t)n_pages * n_kv_heads * page_size * d_head;
+    *code_bytes = dtype == NC_Q8 ? values : 2 * values;
+    *delta_bytes = dtype == NC_Q8 ? values / 32 * 2 : 0;
+    return NC_OK;
+}
+
+int nc_page_pool_init(const nc_page_pool* pool, void* stream)
+{
+    if (int s = check_pool("page_pool_init", pool)) return s;
+    hipLaunchKernelGGL(k_pool_init, dim3((pool->n_pages + 255) / 256), dim3(256), 0, stream_of(stream),
+                       pool->free_pages, pool->state, pool->n_pages);
+    return launch_status("k_pool_init");
+}
+
+int nc_paged_plan(const nc_page_pool* pool, const nc_paged_batch* b, void* stream)
+{
+    if (int s = check_pool("paged_plan", pool)) return s;
+    if (int s = check_batch("paged_plan", b, pool->page_size)) return s;
+    NC_CHECK_ARG(b->new_len && b->seq_len, "paged_plan: null lengths");
+    // the workgroups read the lengths while one of them writes the tables
+    const size_t lens = (size_t)b->n_req * 4, rows = (size_t)b->max_tokens * 4;
+    const void* in[] = {b->new_len, b->seq_len};
+    for (const void* p : in)
+        NC_CHECK_ARG(!overlap(p, lens, b->row_start, lens + 4) && !overlap(p, lens, b->kv_len, lens) &&
+                         !overlap(p, lens, b->positions, rows) && !overlap(p, lens, b->slots, rows),
+                     "paged_plan: a table lies over the lengths");
+    const int grid = b->max_tokens > kPlanRows ? (b->max_tokens + kPlanRows - 1) / kPlanRows : 1;
+    hipLaunchKernelGGL(k_paged_plan, dim3(grid), dim3(kPlanThreads), 0, stream_of(stream), *b, pool->free_pages,
+                       pool->state, pool->n_pages, log2_of(pool->page_size));
+    return launch_status("k_paged_plan");
+}
+
+int nc_paged_commit(const nc_page_pool* pool, const nc_paged_batch* b, const int32_t* finished, void* stream)
+{
+    if (int s = check_pool("paged_commit", pool)) return s;
+    if (int s = check_batch("paged_commit", b, pool->page_size)) return s;
+    NC_CHECK_ARG(b->seq_len, "paged_commit: null lengths");
+    hipLaunchKernelGGL(k_paged_commit, dim3(1), dim3(kCommitThreads), 0, stream_of(stream), *b, pool->free_pages,
+                       pool->state, pool->n_pages, log2_of(pool->page_size), finished);
+    return launch_status("k_paged_commit");
+}
+
+int nc_paged_append(const nc_tensor* q, const nc_tensor* k, const nc_tensor* v, nc_tensor* q_out,
+                    const nc_paged_cache* cache, const nc_paged_batch* b, const float* rope, int rope_rows, int d_half,
+                    void* stream)
+{
+    if (int s = check_cache("paged_append", cache)) return s;
+    if (int s = check_batch("paged_append", b, cache->page_size)) return s;
+    const int d = cache->d_head, kvd = cache->n_kv_heads * d;
+    NC_CHECK_ARG(paged_rows_ok(k, b->max_tokens, kvd) && paged_rows_ok(v, b->max_tokens, kvd) && k->dtype == v->dtype,
+                 "paged_append: k and v are not %d aligned rows of %d values of one type", b->max_tokens, kvd);
+    NC_CHECK_ARG((q == nullptr) == (q_out == nullptr), "paged_append: q and q_out come together");
+    if (q) {
+        NC_CHECK_ARG(q->cols > 0 && q->cols % d == 0 && q->cols / d <= 1024, "paged_append: q of %d values", q->cols);
+        NC_CHECK_ARG(paged_rows_ok(q, b->max_tokens, q->cols) && q->dtype == k->dtype &&
+                         paged_rows_ok(q_out, b->max_tokens, q->cols),
+                     "paged_append: q and q_out are not %d aligned rows, q of k's type", b->max_tokens);
+        NC_CHECK_ARG(q_out->dtype == NC_F16 || q_out->dtype == NC_Q8, "paged_append: q_out dtype %d (F16 or Q8)",
+                     q_out->dtype);
+        if (b->max_tokens && overlap(q->data, (size_t)b->max_tokens * q->pitch, q_out->data,
+                                     (size_t)b->max_tokens * q_out->pitch))
+            NC_CHECK_ARG(q->data == q_out->data && q->dtype == q_out->dtype && q->pitch == q_out->pitch,
+                         "paged_append: q_out lies over q but is not q");
+    }
+    if (rope)
+        NC_CHECK_ARG(rope_rows >= 1 && d_half >= 0 && 2 * d_half <= d && (reinterpret_cast<uintptr_t>(rope) & 7) == 0,
+                     "paged_append: rope table of %d rows, %d pairs of %d values", rope_rows, d_half, d);
+    if (b->max_tokens == 0) return NC_OK;
+    AppendArgs a{};
+    a.hq = q ? q->cols / d : 0;
+    if (q) {
+        a.q = (const uint8_t*)q->data;
+        a.q_pitch = q->pitch;
+        a.q_out = (uint8_t*)q_out->data;
+        a.o_pitch = q_out->pitch;
+    }
+    a.k = (const uint8_t*)k->data;
+    a.k_pitch = k->pitch;
+    a.v = (const uint8_t*)v->data;
+    a.v_pitch = v->pitch;
+    a.kc = (uint8_t*)cache->k;
+    a.vc = (uint8_t*)cache->v;
+    a.kd = (uint16_t*)cache->k_deltas;
+    a.vd = (uint16_t*)cache->v_deltas;
+    a.positions = b->positions;
+    a.slots = b->slots;
+    a.rope = d_half ? reinterpret_cast<const float2*>(rope) : nullptr;
+    a.rope_rows = rope_rows;
+    a.d_half = d_half;
+    a.rows = b->max_tokens;
+    a.hkv = cache->n_kv_heads;
+    a.n_slots = cache->n_pages * cache->page_size;
+    a.lps = log2_of(cache->page_size);
+    const long long threads = (long long)a.rows * (a.hq + 2 * a.hkv) * (d / 8);
+    const long long grid = (threads + 255) / 256;
+    NC_CHECK_ARG(grid <= 0x7FFFFFFFll / 256, "paged_append: %d rows of %d heads are too many", a.rows, a.hq + 2 * a.hkv);
+    const int qdt = q ? q_out->dtype : cache->dtype;
+    hipStream_t st = stream_of(stream);
+    if (k->dtype == NC_Q8) append_launch<Q8>(a, qdt, cache->dtype, d, (unsigned)grid, st);
+    else if (k->dtype == NC_F16) append_launch<F16>(a, qdt, cache->dtype, d, (unsigned)grid, st);
+    else append_launch<F32>(a, qdt, cache->dtype, d, (unsigned)grid, st);
+    return launch_status("k_paged_append");
+}
+
+}  // extern "C"
