@@ -16,10 +16,8 @@
 // operand's slots are permuted alike for both factors, so nothing moves
 // between lanes.
 //
-// Roundings: K, V and Q are fp16 (exact for fp16 tensors; a Q8 code times its
-// delta rounds once, 2^-11 of the value, an eighth of a code's own step at
-// full range), probabilities round to fp16 (2^-11 each; the fp16 result
-// rounds as much), everything else is fp32.  Probabilities are scaled by 2^14
+// Roundings: K, V and Q are fp16, probabilities round to fp16 (2^-11 each;
+// the fp16 result rounds as much), everything else is fp32.  Probabilities are scaled by 2^14
 // so that what falls under fp16's smallest number is below 2^-38 of the
 // maximum's weight.
 #include "nc_act.h"
@@ -105,39 +103,48 @@ __device__ __forceinline__ int page_at(const AttnArgs& a, int req, int pos)
     return (unsigned)id < (unsigned)a.n_pages ? id : -1;
 }
 
-// Four fp16 pairs of eight codes times a delta: a code plus 128 in the low
-// bits of 0x6400 is the fp16 number 1152 + code, so the subtraction is exact
-// and the product rounds once.
-__device__ __forceinline__ half8 dequant8(uint2 c, uint16_t delta)
+// Four codes as fp16 numbers: a code plus 128 in the low bits of 0x6400 is
+// the fp16 number 1152 + code, so the subtraction is exact.
+__device__ __forceinline__ void codes4(uint32_t c, half2v (&v)[2])
 {
     const half2v bias = {(_Float16)-1152.0f, (_Float16)-1152.0f};
+    const uint32_t w = c ^ 0x80808080u;
+    v[0] = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, w, 0x04010400u)) + bias;
+    v[1] = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, w, 0x04030402u)) + bias;
+}
+
+// The products of eight codes and a delta in fp16, rounded once (hi), and
+// what that rounding left (lo; hi + lo is the product, its 18 bits exactly).
+struct HalfPair8 {
+    half8 hi, lo;
+};
+__device__ __forceinline__ HalfPair8 dequant8(uint2 c, uint16_t delta)
+{
     const _Float16 d = __builtin_bit_cast(_Float16, delta);
     const half2v d2 = {d, d};
-    uint32_t out[4];
+    u32x4 hi, lo;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const uint32_t w = (i < 2 ? c.x : c.y) ^ 0x80808080u;
-        const uint32_t p = __builtin_amdgcn_perm(0x64646464u, w, i & 1 ? 0x04030402u : 0x04010400u);
-        out[i] = __builtin_bit_cast(uint32_t, (__builtin_bit_cast(half2v, p) + bias) * d2);
+    for (int i = 0; i < 2; i++) {
+        half2v v[2];
+        codes4(i ? c.y : c.x, v);
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const half2v h = v[j] * d2;
+            hi[2 * i + j] = __builtin_bit_cast(uint32_t, h);
+            lo[2 * i + j] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(v[j], d2, -h));
+        }
     }
-    return __builtin_bit_cast(half8, out);
+    return {__builtin_bit_cast(half8, hi), __builtin_bit_cast(half8, lo)};
 }
 
-
-// Four of them.
-__device__ __forceinline__ uint2 dequant4(uint32_t c, uint16_t delta)
+// Eight values, from col on, of a q row of `cols`.
+template <int QDT>
+__device__ __forceinline__ HalfPair8 q_values(const uint8_t* row, int col, int cols)
 {
-    const half8 h = dequant8(make_uint2(c, 0), delta);
-    const u32x4 w = __builtin_bit_cast(u32x4, h);
-    return make_uint2(w.x, w.y);
-}
-
-// Eight values, from col on, of a q row as fp16.
-__device__ __forceinline__ half8 q_values(const AttnArgs& a, const uint8_t* row, int col, int cols)
-{
-    if (a.q_dtype == F16) return *reinterpret_cast<const half8*>(row + 2 * col);
-    return dequant8(*reinterpret_cast<const uint2*>(row + col),
-                    reinterpret_cast<const uint16_t*>(row + cols)[col >> 5]);
+    if constexpr (QDT == F16) return {*reinterpret_cast<const half8*>(row + 2 * col), half8{}};
+    else
+        return dequant8(*reinterpret_cast<const uint2*>(row + col),
+                        reinterpret_cast<const uint16_t*>(row + cols)[col >> 5]);
 }
 
 // Eight results of one (row, head), from column c8 * 8 of the head on.
@@ -164,15 +171,28 @@ __device__ __forceinline__ f32x4 mfma16(half8 a, half8 b, f32x4 c)
 // from 8 (l / 16) on: the matrix operand as it is loaded.  V: a lane loads
 // d / 16 neighbouring values of the eight positions that its probabilities
 // belong to, one load per position with whole rows across sixteen lanes, and
-// v_perm turns the 8 x d / 16 block into d / 16 operands in registers.
+// v_perm turns the 8 x d / 16 block into d / 16 operands in registers.  The
+// next step's K is requested as soon as this step's is used up, and so its V:
+// the same registers are always in flight or in use.
+//
+// A Q8 value is its code times its delta, 18 bits: here it enters as two
+// fp16 halves, so a Q8 cache adds no rounding of its own.
 
+__device__ __forceinline__ bool pair_not_finite(uint32_t w)
+{
+    return ((w & 0x7C00u) == 0x7C00u) | ((w & 0x7C000000u) == 0x7C000000u);
+}
+
+// Page, rows and lane offsets of one 32-position step.
 template <int D, int CDT>
 struct Kv16 {
     static constexpr int kKs = D / 32;
-    u32x4 k[2][CDT == Q8 ? kKs / 2 : kKs];
-    uint32_t v[8][CDT == Q8 ? D / 64 : D / 32];
-    uint16_t kd[2][CDT == Q8 ? kKs / 2 : 1], vd[CDT == Q8 ? 8 : 1];
-    int page[2];
+    static constexpr int kRow = CDT == Q8 ? D : 2 * D;  // bytes of a row
+    static constexpr int kNk = CDT == Q8 ? kKs / 2 : kKs;
+    static constexpr int kNv = CDT == Q8 ? D / 64 : D / 32;
+    u32x4 k[2][kNk];
+    uint32_t v[8][kNv];
+    uint16_t kd[2][kNk], vd[8];
 
     // First of the eight values that lane group g holds of operand ks.
     static __device__ __forceinline__ int col(int ks, int g)
@@ -180,106 +200,107 @@ struct Kv16 {
         return CDT == Q8 ? (ks >> 1) * 64 + g * 16 + (ks & 1) * 8 : ks * 32 + g * 8;
     }
 
-    __device__ __forceinline__ void load(const AttnArgs& a, int head, int pos, int p0, int p1, int c, int g)
+    // `row`: the cache row of the half step's first position.
+    __device__ __forceinline__ void load_k(const AttnArgs& a, int h, size_t row, int c, int g)
     {
-        page[0] = p0;
-        page[1] = p1;
-        const int mask = (1 << a.lps) - 1;
+        const uint8_t* base = a.k + row * kRow;
+        const uint32_t at = c * kRow + g * 16;
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            // row of the half step's first position
-            const size_t row = ((((size_t)max(page[h], 0) * a.hkv + head) << a.lps) + ((pos + 16 * h) & mask));
-            const size_t kr = row + c;
-            if constexpr (CDT == Q8) {
+        for (int i = 0; i < kNk; i++) k[h][i] = *reinterpret_cast<const u32x4*>(base + (at + i * 64));
+        if constexpr (CDT == Q8) {
+            const uint16_t* db = a.kd + row * (D / 32);
+            const uint32_t dat = c * (D / 32) + (g >> 1);
 #pragma unroll
-                for (int i = 0; i < kKs / 2; i++) {
-                    k[h][i] = *reinterpret_cast<const u32x4*>(a.k + kr * D + i * 64 + g * 16);
-                    kd[h][i] = a.kd[kr * (D / 32) + i * 2 + (g >> 1)];
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < kKs; i++)
-                    k[h][i] = *reinterpret_cast<const u32x4*>(a.k + (kr * D + i * 32 + g * 8) * 2);
-            }
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const size_t vr = row + 4 * g + j;
-                uint32_t* to = v[4 * h + j];
-                if constexpr (CDT == Q8) {
-                    const uint8_t* p = a.v + vr * D + c * (D / 16);
-                    if constexpr (D == 128) {
-                        const uint2 w = *reinterpret_cast<const uint2*>(p);
-                        to[0] = w.x;
-                        to[1] = w.y;
-                    } else {
-                        to[0] = *reinterpret_cast<const uint32_t*>(p);
-                    }
-                    vd[4 * h + j] = a.vd[vr * (D / 32) + c / (512 / D)];
-                } else {
-                    const uint8_t* p = a.v + (vr * D + c * (D / 16)) * 2;
-                    if constexpr (D == 128) {
-                        const u32x4 w = *reinterpret_cast<const u32x4*>(p);
-#pragma unroll
-                        for (int i = 0; i < 4; i++) to[i] = w[i];
-                    } else {
-                        const uint2 w = *reinterpret_cast<const uint2*>(p);
-                        to[0] = w.x;
-                        to[1] = w.y;
-                    }
-                }
-            }
+            for (int i = 0; i < kNk; i++) kd[h][i] = db[dat + 2 * i];
         }
     }
 
-    __device__ __forceinline__ half8 k_operand(int h, int ks) const
+    __device__ __forceinline__ void load_v(const AttnArgs& a, int h, size_t row, int c, int g)
+    {
+        const uint8_t* base = a.v + row * kRow;
+        const uint32_t at = 4 * g * kRow + c * (kRow / 16);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const uint8_t* p = base + (at + j * kRow);
+            if constexpr (kNv == 4) {
+                const u32x4 w = *reinterpret_cast<const u32x4*>(p);
+                v[4 * h + j][0] = w.x, v[4 * h + j][1] = w.y, v[4 * h + j][2] = w.z, v[4 * h + j][3] = w.w;
+            } else if constexpr (kNv == 2) {
+                const uint2 w = *reinterpret_cast<const uint2*>(p);
+                v[4 * h + j][0] = w.x, v[4 * h + j][1] = w.y;
+            } else {
+                v[4 * h + j][0] = *reinterpret_cast<const uint32_t*>(p);
+            }
+        }
+        if constexpr (CDT == Q8) {
+            const uint16_t* db = a.vd + row * (D / 32);
+            const uint32_t dat = 4 * g * (D / 32) + c / (512 / D);
+#pragma unroll
+            for (int j = 0; j < 4; j++) vd[4 * h + j] = db[dat + j * (D / 32)];
+        }
+    }
+
+    __device__ __forceinline__ HalfPair8 k_operand(int h, int ks) const
     {
         if constexpr (CDT == Q8) {
             const u32x4 w = k[h][ks >> 1];
             return dequant8(ks & 1 ? make_uint2(w.z, w.w) : make_uint2(w.x, w.y), kd[h][ks >> 1]);
         } else {
-            return __builtin_bit_cast(half8, k[h][ks]);
+            return {__builtin_bit_cast(half8, k[h][ks]), half8{}};
         }
     }
 
-    // The fp16 values of V, D / 32 pairs per position.
-    __device__ __forceinline__ void v_values(uint32_t (&w)[8][D / 32]) const
+    // Position j's values where `keep` has ones, zeros where it has none.
+    __device__ __forceinline__ void v_clear(int j, uint32_t keep)
     {
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            if constexpr (CDT == F16) {
+        for (int i = 0; i < kNv; i++) v[j][i] &= keep;
+        if constexpr (CDT == Q8) vd[j] &= (uint16_t)keep;
+    }
+
+    // Whether position j may hold an infinity or NaN.
+    __device__ __forceinline__ bool v_not_finite(int j) const
+    {
+        if constexpr (CDT == Q8) return (vd[j] & 0x7FFFu) >= 0x6000u;  // a delta of 512: 128 of them pass fp16
+        bool odd = false;
 #pragma unroll
-                for (int i = 0; i < D / 32; i++) w[j][i] = v[j][i];
-            } else if constexpr (D == 128) {
-                const u32x4 x = __builtin_bit_cast(u32x4, dequant8(make_uint2(v[j][0], v[j][1]), vd[j]));
-#pragma unroll
-                for (int i = 0; i < 4; i++) w[j][i] = x[i];
-            } else {
-                const uint2 x = dequant4(v[j][0], vd[j]);
-                w[j][0] = x.x;
-                w[j][1] = x.y;
-            }
+        for (int i = 0; i < kNv; i++) odd |= pair_not_finite(v[j][i]);
+        return odd;
+    }
+
+    // Pair i (values 2 i and 2 i + 1 of the lane's d / 16) of position j.
+    __device__ __forceinline__ void v_pair(int j, int i, uint32_t& hi, uint32_t& lo) const
+    {
+        if constexpr (CDT == Q8) {
+            const _Float16 d = __builtin_bit_cast(_Float16, vd[j]);
+            const half2v d2 = {d, d};
+            half2v x[2];
+            codes4(v[j][i >> 1], x);
+            const half2v h = x[i & 1] * d2;
+            hi = __builtin_bit_cast(uint32_t, h);
+            lo = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(x[i & 1], d2, -h));
+        } else {
+            hi = v[j][i];
+            lo = 0;
         }
     }
 };
 
-__device__ __forceinline__ bool pair_not_finite(uint32_t w)
-{
-    return (w & 0x7C00u) == 0x7C00u || (w & 0x7C000000u) == 0x7C000000u;
-}
-
-// Operand dt of V^T: value dt of the eight positions.
-template <int D>
-__device__ __forceinline__ half8 v_operand(const uint32_t (&w)[8][D / 32], int dt)
+// Matrix operand of value 2 i + odd of eight positions, from their pairs i.
+__device__ __forceinline__ half8 v_operand(const uint32_t (&w)[8], bool odd)
 {
     u32x4 o;
 #pragma unroll
     for (int i = 0; i < 4; i++)
-        o[i] = __builtin_amdgcn_perm(w[2 * i + 1][dt >> 1], w[2 * i][dt >> 1], dt & 1 ? 0x07060302u : 0x05040100u);
+        o[i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], odd ? 0x07060302u : 0x05040100u);
     return __builtin_bit_cast(half8, o);
 }
 
-template <int D, int CDT>
-__global__ __launch_bounds__(256, 2) void k_paged_attn16(AttnArgs a)
+// MULTI: tiles may hold rows of several tokens, which see different positions.
+// Single tokens have no use for what handles those, and its registers cost
+// them a quarter of the wavefronts.
+template <int D, int CDT, int QDT, bool MULTI>
+__global__ __launch_bounds__(256, D == 64 && !MULTI ? 4 : (D == 64 || !MULTI ? 3 : 2)) void k_paged_attn16(AttnArgs a)
 {
     constexpr int kKs = D / 32, kDt = D / 16, kPitch = D + 4;
     __shared__ float o_sh[4][16][kPitch];
@@ -302,32 +323,61 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn16(AttnArgs a)
 
     // this lane's row: q operand and position
     const int my = min(t.row0 + c, t.n_rows - 1);
-    const int my_tok = my / a.group, my_pos = t.pos0 + my_tok;
-    half8 q[kKs];
+    const int my_tok = my / a.group, my_pos = t.pos0 + my_tok, my_lo = a.window ? my_pos - a.window + 1 : 0;
+    HalfPair8 q[kKs];
     {
         const uint8_t* row = a.q + (size_t)(t.first_row + my_tok) * a.q_pitch;
         const int col = (head * a.group + my % a.group) * D;
 #pragma unroll
-        for (int ks = 0; ks < kKs; ks++) q[ks] = q_values(a, row, col + Kv16<D, CDT>::col(ks, g), a.hq * D);
+        for (int ks = 0; ks < kKs; ks++)
+            q[ks] = q_values<QDT>(row, col + Kv16<D, CDT>::col(ks, g), a.hq * D);
     }
     float m = -__builtin_inff(), sum = 0.0f;
     f32x4 o[kDt];
 #pragma unroll
     for (int i = 0; i < kDt; i++) o[i] = f32x4{0, 0, 0, 0};
 
-    auto fetch = [&](Kv16<D, CDT>& kv, int v) {
-        const int pos = steps.at(v) * 32;
-        kv.load(a, head, pos, page_at(a, req, pos), page_at(a, req, pos + 16), c, g);
+    Kv16<D, CDT> kv;
+    const int mask = (1 << a.lps) - 1;
+    auto row_of = [&](int page, int pos) {
+        return (((size_t)max(page, 0) * a.hkv + head) << a.lps) + (pos & mask);
     };
-    auto use = [&](const Kv16<D, CDT>& kv, int v) {
-        const int pos = steps.at(v) * 32;
+    int v = v0 + wave;
+    int pos = 0, p0 = 0, p1 = 0;
+    if (v < v1) {
+        pos = steps.at(v) * 32;
+        p0 = page_at(a, req, pos);
+        p1 = page_at(a, req, pos + 16);
+        kv.load_k(a, 0, row_of(p0, pos), c, g);
+        kv.load_k(a, 1, row_of(p1, pos + 16), c, g);
+        kv.load_v(a, 0, row_of(p0, pos), c, g);
+        kv.load_v(a, 1, row_of(p1, pos + 16), c, g);
+    }
+    while (v < v1) {
+        const int nv = v + 4;
+        int npos = 0, np0 = 0, np1 = 0;
+        if (nv < v1) {
+            npos = steps.at(nv) * 32;
+            np0 = page_at(a, req, npos);
+            np1 = page_at(a, req, npos + 16);
+        }
         f32x4 s[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
 #pragma unroll
         for (int ks = 0; ks < kKs; ks++)
 #pragma unroll
-            for (int h = 0; h < 2; h++) s[h] = mfma16(kv.k_operand(h, ks), q[ks], s[h]);
+            for (int h = 0; h < 2; h++) {
+                const HalfPair8 k = kv.k_operand(h, ks);
+                s[h] = mfma16(k.hi, q[ks].hi, s[h]);
+                if constexpr (CDT == Q8) s[h] = mfma16(k.lo, q[ks].hi, s[h]);
+                if constexpr (QDT == Q8) s[h] = mfma16(k.hi, q[ks].lo, s[h]);
+            }
+        __builtin_amdgcn_sched_barrier(0);
+        if (nv < v1) {
+            kv.load_k(a, 0, row_of(np0, npos), c, g);
+            kv.load_k(a, 1, row_of(np1, npos + 16), c, g);
+        }
         const int last = t.pos0 + t.tok_hi;
-        const bool all = pos + 31 <= t.pos0 + t.tok_lo && kv.page[0] >= 0 && kv.page[1] >= 0 &&
+        const bool all = pos + 31 <= t.pos0 + t.tok_lo && p0 >= 0 && p1 >= 0 &&
                          (!a.window || pos > last - a.window || pos + 31 < a.sink);
         float x[8];
 #pragma unroll
@@ -336,9 +386,8 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn16(AttnArgs a)
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const int key = pos + 16 * (j >> 2) + 4 * g + (j & 3);
-                const bool seen = key <= my_pos && (!a.window || key > my_pos - a.window || key < a.sink) &&
-                                  kv.page[j >> 2] >= 0;
-                if (!seen) x[j] = -__builtin_inff();
+                const bool seen = (key <= my_pos) & ((key >= my_lo) | (key < a.sink)) & ((j < 4 ? p0 : p1) >= 0);
+                x[j] = seen ? x[j] : -__builtin_inff();
             }
         }
         float mx = x[0];
@@ -363,61 +412,75 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn16(AttnArgs a)
 #pragma unroll
             for (int i = 0; i < kDt; i++) o[i] *= alpha;
         }
-        uint32_t w[8][D / 32];
-        kv.v_values(w);
-        bool odd = false;  // a value that no probability of 0 can hide
+        // O^T += V^T P^T; positions that no row of the tile sees are cleared,
+        // for a probability of 0 does not hide an infinity or NaN
+        bool by_token = false;
         if (!all) {
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const int key = pos + 16 * (j >> 2) + 4 * g + (j & 3);
-                const bool seen = key < t.hi && (!a.window || key >= t.lo || key < a.sink) && kv.page[j >> 2] >= 0;
+                const bool seen = (key < t.hi) & ((key >= t.lo) | (key < a.sink)) & ((j < 4 ? p0 : p1) >= 0);
+                kv.v_clear(j, seen ? ~0u : 0u);
+            }
+            if (MULTI && t.tok_lo != t.tok_hi) {
+                bool odd = false;
 #pragma unroll
-                for (int i = 0; i < D / 32; i++) {
-                    if (!seen) w[j][i] = 0;
-                    odd |= pair_not_finite(w[j][i]);
-                }
+                for (int j = 0; j < 8; j++) odd |= kv.v_not_finite(j);
+                by_token = __ballot(odd) != 0;
             }
         }
-        if (!all && t.tok_lo != t.tok_hi && __ballot(odd)) {
+        if (!by_token) {
+#pragma unroll
+            for (int i = 0; i < kDt / 2; i++) {
+                uint32_t hi[8], lo[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) kv.v_pair(j, i, hi[j], lo[j]);
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    o[2 * i + e] = mfma16(v_operand(hi, e), p, o[2 * i + e]);
+                    if constexpr (CDT == Q8) o[2 * i + e] = mfma16(v_operand(lo, e), p, o[2 * i + e]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        } else {
             // positions that some of the tile's rows see and others do not
-            // hold infinities or NaN: one token after the other, with its
-            // unseen positions' values cleared
+            // hold infinities or NaN: one token after the other, with the
+            // values of the positions that it does not see cleared
             for (int tok = t.tok_lo; tok <= t.tok_hi; tok++) {
-                const int at = t.pos0 + tok;
-                uint32_t u[8][D / 32];
+                const int at = t.pos0 + tok, at_lo = a.window ? at - a.window + 1 : 0;
+                uint32_t mine[8];
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     const int key = pos + 16 * (j >> 2) + 4 * g + (j & 3);
-                    const bool seen = key <= at && (!a.window || key > at - a.window || key < a.sink);
-#pragma unroll
-                    for (int i = 0; i < D / 32; i++) u[j][i] = seen ? w[j][i] : 0;
+                    mine[j] = (key <= at) & ((key >= at_lo) | (key < a.sink)) ? ~0u : 0u;
                 }
 #pragma unroll
-                for (int i = 0; i < kDt; i++) {
-                    const f32x4 r = mfma16(v_operand<D>(u, i), p, o[i]);
-                    if (my_tok == tok) o[i] = r;
+                for (int i = 0; i < kDt / 2; i++) {
+                    uint32_t hi[8], lo[8];
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        kv.v_pair(j, i, hi[j], lo[j]);
+                        hi[j] &= mine[j];
+                        lo[j] &= mine[j];
+                    }
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        f32x4 r = mfma16(v_operand(hi, e), p, o[2 * i + e]);
+                        if constexpr (CDT == Q8) r = mfma16(v_operand(lo, e), p, r);
+                        if (my_tok == tok) o[2 * i + e] = r;
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
-            return;
         }
-#pragma unroll
-        for (int i = 0; i < kDt; i++) o[i] = mfma16(v_operand<D>(w, i), p, o[i]);
-    };
-
-    // two steps' loads in flight
-    {
-        Kv16<D, CDT> x, y;
-        int v = v0 + wave;
-        if (v < v1) fetch(x, v);
-        while (v < v1) {
-            if (v + 4 < v1) fetch(y, v + 4);
-            use(x, v);
-            v += 4;
-            if (v >= v1) break;
-            if (v + 4 < v1) fetch(x, v + 4);
-            use(y, v);
-            v += 4;
+        if (nv < v1) {
+            kv.load_v(a, 0, row_of(np0, npos), c, g);
+            kv.load_v(a, 1, row_of(np1, npos + 16), c, g);
         }
+        v = nv;
+        pos = npos;
+        p0 = np0;
+        p1 = np1;
     }
     sum += __shfl_xor(sum, 16);
     sum += __shfl_xor(sum, 32);
@@ -567,7 +630,15 @@ static int attn_launch(const AttnArgs& a, hipStream_t st)
 {
     const long long tiles = (long long)a.n_req * a.row_tiles * a.hkv;
     NC_CHECK_ARG(tiles * a.splits * 256 <= 0x7FFFFFFFll * 2, "paged_attn: %lld tiles are too many", tiles);
-    hipLaunchKernelGGL((k_paged_attn16<D, CDT>), dim3((unsigned)(tiles * a.splits)), dim3(256), 0, st, a);
+    const dim3 grid((unsigned)(tiles * a.splits));
+    const bool multi = a.max_new > 1;
+    if (a.q_dtype == F16) {
+        if (multi) hipLaunchKernelGGL((k_paged_attn16<D, CDT, F16, true>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((k_paged_attn16<D, CDT, F16, false>), grid, dim3(256), 0, st, a);
+    } else {
+        if (multi) hipLaunchKernelGGL((k_paged_attn16<D, CDT, Q8, true>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((k_paged_attn16<D, CDT, Q8, false>), grid, dim3(256), 0, st, a);
+    }
     if (a.splits > 1) hipLaunchKernelGGL((k_paged_join<D>), dim3((unsigned)tiles), dim3(16 * D / 8), 0, st, a);
     return launch_status("k_paged_attn16");
 }
