@@ -43,10 +43,12 @@ struct AttnArgs {
     int hq, hkv, group, max_tokens, max_new, max_kv;
     int window, sink;
     float scale;   // log2(e) / sqrt(d)
-    int row_tiles; // tiles of a request, or tile slots in all
-    int splits;    // parts of a tile's positions at most
-    int part;      // steps of a part
-    float* ws;     // [splits][max_tokens * hq][d] sums, then [splits][max_tokens * hq][2] (maximum, sum)
+    int few;        // requests of at most this many (token, head) rows take sixteen-row tiles
+    int row_tiles;  // sixteen-row tiles of a request
+    int splits;     // parts of a tile's positions at most
+    int part;       // steps of a part
+    int splits_max; // of all the call's launches
+    float* ws;      // [splits_max][max_tokens * hq][d] sums, then as many (maximum, sum) pairs
 };
 
 // The positions that a tile of rows visits, in steps of S: [0, n_sink) and
@@ -94,6 +96,17 @@ __device__ __forceinline__ bool tile_of(const AttnArgs& a, int req, int row0, Ti
     t.hi = t.pos0 + t.tok_hi + 1;
     return true;
 }
+
+// The positions besides the sinks whose values count: all that the tile's rows
+// see, or those of one of its tokens.
+struct Seen {
+    int lo, hi;
+    __device__ __forceinline__ Seen(const AttnArgs& a, const Tile& t, int token)
+    {
+        hi = token < 0 ? t.hi : t.pos0 + token + 1;
+        lo = token < 0 ? t.lo : (a.window ? max(0, hi - a.window) : 0);
+    }
+};
 
 // A page id, or -1 for an entry that is none: callers read page 0 in its
 // place and take its positions for unseen.
@@ -296,15 +309,13 @@ __device__ __forceinline__ half8 v_operand(const uint32_t (&w)[8], bool odd)
     return __builtin_bit_cast(half8, o);
 }
 
-// MULTI: tiles may hold rows of several tokens, which see different positions.
-// Single tokens have no use for what handles those, and its registers cost
-// them a quarter of the wavefronts.
-template <int D, int CDT, int QDT, bool MULTI>
-__global__ __launch_bounds__(256, D == 64 && !MULTI ? 4 : (D == 64 || !MULTI ? 3 : 2)) void k_paged_attn16(AttnArgs a)
+template <int D, int CDT, int QDT>
+__global__ __launch_bounds__(256, D == 64 ? 4 : 3) void k_paged_attn16(AttnArgs a)
 {
     constexpr int kKs = D / 32, kDt = D / 16, kPitch = D + 4;
     __shared__ float o_sh[4][16][kPitch];
     __shared__ float ml_sh[4][16][2];
+    __shared__ int odd_sh;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 15, g = lane >> 4;
     int b = blockIdx.x;
@@ -314,8 +325,8 @@ __global__ __launch_bounds__(256, D == 64 && !MULTI ? 4 : (D == 64 || !MULTI ? 3
     b /= a.hkv;
     const int req = b / a.row_tiles;
     Tile t;
-    if (!tile_of<16>(a, req, (b % a.row_tiles) * 16, t)) return;
-    const Steps<32> steps(t.lo, t.hi, a.window ? a.sink : 0);
+    if (!tile_of<16>(a, req, (b % a.row_tiles) * 16, t) || t.n_rows > a.few) return;
+    const Steps<32> steps(t.lo, t.hi, a.sink);
     const int v0 = part * a.part;
     if (v0 >= steps.count) return;
     const int v1 = part == a.splits - 1 ? steps.count : min(v0 + a.part, steps.count);
@@ -332,6 +343,15 @@ __global__ __launch_bounds__(256, D == 64 && !MULTI ? 4 : (D == 64 || !MULTI ? 3
         for (int ks = 0; ks < kKs; ks++)
             q[ks] = q_values<QDT>(row, col + Kv16<D, CDT>::col(ks, g), a.hq * D);
     }
+    if (tid == 0) odd_sh = 0;
+    __syncthreads();
+
+    // Once for all tokens; where a position that some of the tile's rows see
+    // and others do not holds an infinity or NaN, which a probability of 0
+    // does not hide, once more for each token, with the values of all
+    // positions that it does not see cleared.
+    for (int only = -1;;) {
+    const Seen see(a, t, only);
     float m = -__builtin_inff(), sum = 0.0f;
     f32x4 o[kDt];
 #pragma unroll
@@ -414,64 +434,28 @@ __global__ __launch_bounds__(256, D == 64 && !MULTI ? 4 : (D == 64 || !MULTI ? 3
         }
         // O^T += V^T P^T; positions that no row of the tile sees are cleared,
         // for a probability of 0 does not hide an infinity or NaN
-        bool by_token = false;
         if (!all) {
+            bool odd = false;
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const int key = pos + 16 * (j >> 2) + 4 * g + (j & 3);
-                const bool seen = (key < t.hi) & ((key >= t.lo) | (key < a.sink)) & ((j < 4 ? p0 : p1) >= 0);
+                const bool seen = (key < see.hi) & ((key >= see.lo) | (key < a.sink)) & ((j < 4 ? p0 : p1) >= 0);
                 kv.v_clear(j, seen ? ~0u : 0u);
+                odd |= kv.v_not_finite(j);
             }
-            if (MULTI && t.tok_lo != t.tok_hi) {
-                bool odd = false;
-#pragma unroll
-                for (int j = 0; j < 8; j++) odd |= kv.v_not_finite(j);
-                by_token = __ballot(odd) != 0;
-            }
+            if (odd) odd_sh = 1;
         }
-        if (!by_token) {
 #pragma unroll
-            for (int i = 0; i < kDt / 2; i++) {
-                uint32_t hi[8], lo[8];
+        for (int i = 0; i < kDt / 2; i++) {
+            uint32_t hi[8], lo[8];
 #pragma unroll
-                for (int j = 0; j < 8; j++) kv.v_pair(j, i, hi[j], lo[j]);
+            for (int j = 0; j < 8; j++) kv.v_pair(j, i, hi[j], lo[j]);
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    o[2 * i + e] = mfma16(v_operand(hi, e), p, o[2 * i + e]);
-                    if constexpr (CDT == Q8) o[2 * i + e] = mfma16(v_operand(lo, e), p, o[2 * i + e]);
-                }
-                __builtin_amdgcn_sched_barrier(0);
+            for (int e = 0; e < 2; e++) {
+                o[2 * i + e] = mfma16(v_operand(hi, e), p, o[2 * i + e]);
+                if constexpr (CDT == Q8) o[2 * i + e] = mfma16(v_operand(lo, e), p, o[2 * i + e]);
             }
-        } else {
-            // positions that some of the tile's rows see and others do not
-            // hold infinities or NaN: one token after the other, with the
-            // values of the positions that it does not see cleared
-            for (int tok = t.tok_lo; tok <= t.tok_hi; tok++) {
-                const int at = t.pos0 + tok, at_lo = a.window ? at - a.window + 1 : 0;
-                uint32_t mine[8];
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const int key = pos + 16 * (j >> 2) + 4 * g + (j & 3);
-                    mine[j] = (key <= at) & ((key >= at_lo) | (key < a.sink)) ? ~0u : 0u;
-                }
-#pragma unroll
-                for (int i = 0; i < kDt / 2; i++) {
-                    uint32_t hi[8], lo[8];
-#pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        kv.v_pair(j, i, hi[j], lo[j]);
-                        hi[j] &= mine[j];
-                        lo[j] &= mine[j];
-                    }
-#pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        f32x4 r = mfma16(v_operand(hi, e), p, o[2 * i + e]);
-                        if constexpr (CDT == Q8) r = mfma16(v_operand(lo, e), p, r);
-                        if (my_tok == tok) o[2 * i + e] = r;
-                    }
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-            }
+            __builtin_amdgcn_sched_barrier(0);
         }
         if (nv < v1) {
             kv.load_v(a, 0, row_of(np0, npos), c, g);
@@ -495,8 +479,14 @@ __global__ __launch_bounds__(256, D == 64 && !MULTI ? 4 : (D == 64 || !MULTI ? 3
         ml_sh[wave][c][1] = sum;
     }
     __syncthreads();
+    if (only < 0 && odd_sh && t.tok_lo != t.tok_hi) {
+        only = t.tok_lo;
+        __syncthreads();
+        continue;
+    }
     const int rr = tid / (D / 8), c8 = tid % (D / 8);
-    if (rr >= 16 || t.row0 + rr >= t.n_rows) return;  // whole heads
+    const int row = t.row0 + rr, tok = t.first_row + row / a.group, qh = head * a.group + row % a.group;
+    if (rr < 16 && row < t.n_rows && (only < 0 || only == row / a.group)) {  // whole heads
     float mw[4], top = -__builtin_inff(), total = 0.0f, r[8] = {};
 #pragma unroll
     for (int w = 0; w < 4; w++) top = fmaxf(top, mw[w] = ml_sh[w][rr][0]);
@@ -507,41 +497,401 @@ __global__ __launch_bounds__(256, D == 64 && !MULTI ? 4 : (D == 64 || !MULTI ? 3
 #pragma unroll
         for (int i = 0; i < 8; i++) r[i] += f * o_sh[w][rr][c8 * 8 + i];
     }
-    const int row = t.row0 + rr, tok = t.first_row + row / a.group, qh = head * a.group + row % a.group;
     if (parts == 1) {
         const float inv = total != 0.0f ? 1.0f / total : 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; i++) r[i] *= inv;
         store_out<D>(a, tok, qh, c8, r);
-        return;
-    }
+    } else {
     const size_t rows = (size_t)a.max_tokens * a.hq, at = part * rows + (size_t)tok * a.hq + qh;
     float4* dst = reinterpret_cast<float4*>(a.ws + at * D + c8 * 8);
     dst[0] = make_float4(r[0], r[1], r[2], r[3]);
     dst[1] = make_float4(r[4], r[5], r[6], r[7]);
     if (c8 == 0) {
-        float* ml = a.ws + a.splits * rows * D + at * 2;
+        float* ml = a.ws + a.splits_max * rows * D + at * 2;
         ml[0] = top;
         ml[1] = total;
     }
+    }
+    }
+    if (only < 0 || only == t.tok_hi) return;
+    only++;
+    __syncthreads();
+    }
 }
 
-// The parts of a tile joined in their order.
+// ---- 128 rows a tile -----------------------------------------------------------
+//
+// One workgroup of four wavefronts per (tile, kv head, part of the
+// positions), 32 rows a wavefront, over steps of 64 (d = 128: 32) positions whose K and V
+// all four read from shared memory: each value comes from memory once per 128
+// rows.  The step after the one at work is already on its way to registers,
+// and goes to the other of two buffers while the step is at work: one barrier
+// a step.  V is turned into V^T on its way (a thread turns four positions by
+// four values), its positions in the order in which a lane's probabilities
+// lie in the operand: groups of four at 0, 8, 4, 12 of every sixteen.
+// Sixteen-byte pieces of both are exchanged within rows by a function of the
+// row, so that sixteen neighbouring lanes' reads spread over all banks.
+//
+// Q8 values and q rows enter as their fp16 products, rounded once (2^-11).
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ f32x16 mfma32(half8 a, half8 b, f32x16 c)
+{
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+constexpr int kRowsM = 128;
+constexpr int rows_step(int d) { return d == 128 ? 32 : 64; }  // positions of a step
+
+// Byte offsets in shared memory: K piece (16 bytes) `c` of position `key`;
+// V^T piece `c` (eight positions) of value d.
 template <int D>
+__device__ __forceinline__ int k_place(int key, int c)
+{
+    const int turn = D == 128 ? key & 15 : (key >> 1) & 7;
+    return key * 2 * D + ((c ^ turn) << 4);
+}
+template <int D>
+__device__ __forceinline__ int v_place(int d, int c)
+{
+    const int turn = rows_step(D) == 32 ? (d >> 2) & 3 : ((d >> 1) ^ (d >> 3)) & 7;
+    return d * 2 * rows_step(D) + ((c ^ turn) << 4);
+}
+
+// The pages of a step's sixteens of positions, uniform over a wavefront.
+template <int S>
+struct StepPages {
+    int id[S / 16];
+    __device__ __forceinline__ StepPages(const AttnArgs& a, int req, int pos)
+    {
+#pragma unroll
+        for (int i = 0; i < S / 16; i++) id[i] = page_at(a, req, pos + 16 * i);
+    }
+    __device__ __forceinline__ bool all() const
+    {
+        bool ok = true;
+#pragma unroll
+        for (int i = 0; i < S / 16; i++) ok &= id[i] >= 0;
+        return ok;
+    }
+};
+
+// One thread's share of a step's K and V, on its way through registers.
+template <int D, int CDT>
+struct KvRows {
+    static constexpr int kS = rows_step(D);
+    static constexpr int kNk = D * kS / 8 / 256;  // pieces of eight K values
+    static constexpr int kE = 4;                  // V values of each of four positions
+    static constexpr int kDg = D / kE;            // threads of a position's values
+    u32x4 k[CDT == F16 ? kNk : 1];
+    uint2 kc[CDT == Q8 ? kNk : 1];
+    uint16_t kd[CDT == Q8 ? kNk : 1];
+    uint2 v[CDT == F16 ? 4 : 1];
+    uint32_t vc[CDT == Q8 ? 4 : 1];
+    uint16_t vd[4];
+    uint32_t v_keep;  // a bit for each of the four positions that is to be seen
+    bool partial;     // some of the tile's rows do not see the whole step
+
+    __device__ __forceinline__ void load(const AttnArgs& a, const Tile& t, const Seen& see, const StepPages<kS>& pages,
+                                         int head, int pos, int wave)
+    {
+        const int tid = threadIdx.x, mask = (1 << a.lps) - 1;
+        partial = pos + kS - 1 > t.pos0 + t.tok_lo ||
+                  (a.window && pos <= t.pos0 + t.tok_hi - a.window && pos + kS - 1 >= a.sink);
+        // a wavefront's positions lie in one sixteen, whose first row is
+        auto row_of = [&](int group) {
+            int id = pages.id[0];
+#pragma unroll
+            for (int i = 1; i < kS / 16; i++) id = group == i ? pages.id[i] : id;
+            return (((size_t)max(id, 0) * a.hkv + head) << a.lps) + ((pos + 16 * group) & mask);
+        };
+#pragma unroll
+        for (int i = 0; i < kNk; i++) {
+            const int first = i * 2048 / D + wave * 512 / D;  // of the wavefront's positions
+            const size_t row = row_of(first >> 4);
+            const uint32_t at = (first & 15) + (tid & 63) / (D / 8), c = tid % (D / 8);
+            if constexpr (CDT == F16) {
+                k[i] = *reinterpret_cast<const u32x4*>(a.k + row * (2 * D) + (at * D + c * 8) * 2);
+            } else {
+                kc[i] = *reinterpret_cast<const uint2*>(a.k + row * D + (at * D + c * 8));
+                kd[i] = (a.kd + row * (D / 32))[at * (D / 32) + (c >> 2)];
+            }
+        }
+        const int first = wave * (64 / kDg) * 4, quad = (tid & 63) / kDg;
+        const size_t row = row_of(first >> 4);
+        bool page = pages.id[0] >= 0;
+#pragma unroll
+        for (int i = 1; i < kS / 16; i++) page = first >> 4 == i ? pages.id[i] >= 0 : page;
+        const uint32_t at = (first & 15) + quad * 4, dg = tid % kDg;
+        v_keep = 0;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int p = pos + first + quad * 4 + j;
+            if (page & (p < see.hi) & ((p >= see.lo) | (p < a.sink))) v_keep |= 1u << j;
+            if constexpr (CDT == F16) {
+                v[j] = *reinterpret_cast<const uint2*>(a.v + row * (2 * D) + ((at + j) * D + dg * kE) * 2);
+            } else {
+                vc[j] = *reinterpret_cast<const uint32_t*>(a.v + row * D + ((at + j) * D + dg * kE));
+                vd[j] = (a.vd + row * (D / 32))[(at + j) * (D / 32) + dg * kE / 32];
+            }
+        }
+    }
+
+    // To shared memory; *not_finite = 1 where rows that see a value that is
+    // no number and rows that do not may meet.
+    __device__ __forceinline__ void store(uint8_t* kb, uint8_t* vb, int* not_finite) const
+    {
+        const int tid = threadIdx.x;
+#pragma unroll
+        for (int i = 0; i < kNk; i++) {
+            const int at = i * 256 + tid, key = at / (D / 8), c = at % (D / 8);
+            u32x4 w;
+            if constexpr (CDT == F16) w = k[i];
+            else w = __builtin_bit_cast(u32x4, dequant8(kc[i], kd[i]).hi);
+            *reinterpret_cast<u32x4*>(kb + k_place<D>(key, c)) = w;
+        }
+        uint2 w[4];
+        bool odd = false;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if constexpr (CDT == F16) {
+                w[j] = v[j];
+            } else {
+                const _Float16 d = __builtin_bit_cast(_Float16, vd[j]);
+                half2v x[2];
+                codes4(vc[j], x);
+                w[j] = make_uint2(__builtin_bit_cast(uint32_t, x[0] * half2v{d, d}),
+                                  __builtin_bit_cast(uint32_t, x[1] * half2v{d, d}));
+            }
+            if (partial) {
+                const uint32_t keep = (v_keep >> j) & 1 ? ~0u : 0u;
+                w[j].x &= keep;
+                w[j].y &= keep;
+                odd |= pair_not_finite(w[j].x) | pair_not_finite(w[j].y);
+            } else if (!((v_keep >> j) & 1)) {
+                w[j] = make_uint2(0, 0);  // no page
+            }
+        }
+        if (odd) *not_finite = 1;
+        const int dg = tid % kDg, quad = tid / kDg;  // four positions: the piece and its half
+        const int c = (quad >> 2) * 2 + (quad & 1), half = (quad >> 1) & 1;
+#pragma unroll
+        for (int e = 0; e < kE; e++) {
+            const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
+            const uint32_t x0 = e < 2 ? w[0].x : w[0].y, x1 = e < 2 ? w[1].x : w[1].y;
+            const uint32_t x2 = e < 2 ? w[2].x : w[2].y, x3 = e < 2 ? w[3].x : w[3].y;
+            *reinterpret_cast<uint2*>(vb + v_place<D>(dg * kE + e, c) + half * 8) =
+                make_uint2(__builtin_amdgcn_perm(x1, x0, sel), __builtin_amdgcn_perm(x3, x2, sel));
+        }
+    }
+};
+
+template <int D, int CDT, int QDT>
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_paged_rows(AttnArgs a)
+{
+    constexpr int kS = rows_step(D), kU = kS / 32, kKs = D / 16, kDt = D / 32, kBytes = kS * D * 2;
+    __shared__ __align__(16) uint8_t k_sh[2][kBytes];
+    __shared__ __align__(16) uint8_t v_sh[2][kBytes];
+    __shared__ int odd_sh;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c = lane & 31, h = lane >> 5;
+    int b = blockIdx.x;
+    const int head = b % a.hkv;
+    b /= a.hkv;
+    const int part = b % a.splits;
+    const int slot = b / a.splits;
+    const int req = tile_request(a.row_start, a.n_req, slot, a.group, kRowsM, a.max_tokens);
+    const int row0 = (slot - first_tile(a.row_start[req], req, a.group, kRowsM, a.max_tokens)) * kRowsM;
+    Tile t;
+    if (row0 < 0 || !tile_of<kRowsM>(a, req, row0, t) || t.n_rows <= a.few) return;
+    const Steps<kS> steps(t.lo, t.hi, a.sink);
+    const int v0 = part * a.part;
+    if (v0 >= steps.count) return;
+    const int v1 = part == a.splits - 1 ? steps.count : min(v0 + a.part, steps.count);
+    const int parts = min((steps.count + a.part - 1) / a.part, a.splits);
+
+    const int first = row0 + wave * 32;  // the wavefront's rows
+    const bool mine = first < t.n_rows;
+    const int my = min(first + c, t.n_rows - 1);
+    const int my_tok = my / a.group, my_pos = t.pos0 + my_tok, my_lo = a.window ? my_pos - a.window + 1 : 0;
+    const int w_lo = min(first, t.n_rows - 1) / a.group, w_hi = min(first + 31, t.n_rows - 1) / a.group;
+    half8 q[kKs];
+    {
+        const uint8_t* row = a.q + (size_t)(t.first_row + my_tok) * a.q_pitch;
+        const int col = (head * a.group + my % a.group) * D;
+#pragma unroll
+        for (int ks = 0; ks < kKs; ks++) q[ks] = q_values<QDT>(row, col + ks * 16 + h * 8, a.hq * D).hi;
+    }
+    if (tid == 0) odd_sh = 0;
+    __syncthreads();
+
+    // Once for all tokens.  Where a position that some of the tile's rows see
+    // and others do not holds an infinity or NaN, which a probability of 0
+    // does not hide, once more for each token, with the values of all
+    // positions that it does not see cleared.
+    for (int only = -1;;) {
+    const Seen see(a, t, only);
+    float m = -__builtin_inff(), sum = 0.0f;
+    f32x16 o[kDt];
+#pragma unroll
+    for (int i = 0; i < kDt; i++) o[i] = f32x16{};
+
+    KvRows<D, CDT> kv;
+    StepPages<kS> here(a, req, steps.at(v0) * kS), next(a, req, steps.at(min(v0 + 1, v1 - 1)) * kS);
+    kv.load(a, t, see, here, head, steps.at(v0) * kS, wave);
+    kv.store(k_sh[0], v_sh[0], &odd_sh);
+    __syncthreads();
+    for (int v = v0; v < v1; v++) {
+        const int buf = (v - v0) & 1, pos = steps.at(v) * kS;
+        if (v + 1 < v1) kv.load(a, t, see, next, head, steps.at(v + 1) * kS, wave);
+        const StepPages<kS> after(a, req, steps.at(min(v + 2, v1 - 1)) * kS);
+        // unless the wavefront sees none of the step's positions
+        if (mine && pos <= t.pos0 + w_hi) {
+            const uint8_t *kb = k_sh[buf], *vb = v_sh[buf];
+            f32x16 s[kU];
+#pragma unroll
+            for (int u = 0; u < kU; u++) s[u] = f32x16{};
+#pragma unroll
+            for (int ks = 0; ks < kKs; ks++)
+#pragma unroll
+                for (int u = 0; u < kU; u++)
+                    s[u] = mfma32(*reinterpret_cast<const half8*>(kb + k_place<D>(u * 32 + c, ks * 2 + h)), q[ks], s[u]);
+            const bool pages = here.all();
+            const bool all = pages & (pos + kS - 1 <= t.pos0 + w_lo) &
+                             ((a.window == 0) | (pos > t.pos0 + w_hi - a.window) | (pos + kS - 1 < a.sink));
+            if (!all) {
+                // against the lane's first position: its others lie at constants
+                const int at0 = pos + 4 * h, hi = my_pos - at0, lo = my_lo - at0, sk = a.sink - at0;
+#pragma unroll
+                for (int i = 0; i < 16 * kU; i++) {
+                    const int at = (i >> 4) * 32 + ((i >> 2) & 3) * 8 + (i & 3);
+                    const bool seen = (at <= hi) & ((at >= lo) | (at < sk)) & (here.id[at >> 4] >= 0);
+                    s[i >> 4][i & 15] = seen ? s[i >> 4][i & 15] : -__builtin_inff();
+                }
+            }
+            float mx = s[0][0];
+#pragma unroll
+            for (int i = 1; i < 16 * kU; i++) mx = fmaxf(mx, s[i >> 4][i & 15]);
+            mx = fmaxf(mx, __shfl_xor(mx, 32)) * a.scale;
+            const float m_new = fmaxf(m, mx);
+            const float base = m_new == -__builtin_inff() ? 0.0f : m_new - kPScale;
+            const float alpha = __builtin_amdgcn_exp2f(m - kPScale - base);
+            half8 p[2 * kU];
+            float add = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16 * kU; i++) {
+                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 4][i & 15], a.scale, -base));
+                add += e;
+                p[i >> 3][i & 7] = (_Float16)e;
+            }
+            sum = __builtin_fmaf(sum, alpha, add);
+            m = m_new;
+            if (__ballot(alpha != 1.0f)) {
+#pragma unroll
+                for (int i = 0; i < kDt; i++) o[i] *= alpha;
+            }
+#pragma unroll
+            for (int dt = 0; dt < kDt; dt++)
+#pragma unroll
+                for (int ks = 0; ks < 2 * kU; ks++)
+                    o[dt] = mfma32(*reinterpret_cast<const half8*>(vb + v_place<D>(dt * 32 + c, ks * 2 + h)), p[ks], o[dt]);
+        }
+        // the other buffer was last read before the last barrier
+        if (v + 1 < v1) kv.store(k_sh[buf ^ 1], v_sh[buf ^ 1], &odd_sh);
+        __syncthreads();
+        here = next;
+        next = after;
+    }
+    sum += __shfl_xor(sum, 32);
+    if (only < 0 && odd_sh && t.tok_lo != t.tok_hi) {
+        only = t.tok_lo;
+        continue;
+    }
+    if (first + c < t.n_rows && (only < 0 || only == my_tok)) {
+
+    // lane (c, h): row c, values 32 dt + 8 j + 4 h + i
+    const int tok = t.first_row + my_tok, qh = head * a.group + my % a.group;
+    if (parts > 1) {
+        const size_t rows = (size_t)a.max_tokens * a.hq, at = part * rows + (size_t)tok * a.hq + qh;
+#pragma unroll
+        for (int dt = 0; dt < kDt; dt++)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                *reinterpret_cast<float4*>(a.ws + at * D + dt * 32 + j * 8 + h * 4) =
+                    make_float4(o[dt][4 * j], o[dt][4 * j + 1], o[dt][4 * j + 2], o[dt][4 * j + 3]);
+        if (h == 0) *reinterpret_cast<float2*>(a.ws + a.splits_max * rows * D + at * 2) = make_float2(m, sum);
+    } else {
+    const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+    uint8_t* op = a.out + (size_t)tok * a.out_pitch;
+#pragma unroll
+    for (int dt = 0; dt < kDt; dt++) {
+        if (a.out_dtype == F16) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                float v[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) v[i] = o[dt][4 * j + i] * inv;
+                *reinterpret_cast<uint2*>(op + (qh * D + dt * 32 + j * 8 + h * 4) * 2) =
+                    make_uint2((uint32_t)f2h(v[0]) | (uint32_t)f2h(v[1]) << 16,
+                               (uint32_t)f2h(v[2]) | (uint32_t)f2h(v[3]) << 16);
+            }
+        } else {
+            // q8_quantize of a block whose halves two lanes hold
+            float top = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; i++) top = fmaxf(top, fabsf(o[dt][i] * inv));
+            top = fmaxf(top, __shfl_xor(top, 32));
+            const float delta = top / 127.0f, by = delta != 0.0f ? 1.0f / delta : 0.0f;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                uint32_t w = 0;
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    w |= (uint32_t)(uint8_t)(int8_t)roundf(o[dt][4 * j + i] * inv * by) << (8 * i);
+                *reinterpret_cast<uint32_t*>(op + qh * D + dt * 32 + j * 8 + h * 4) = w;
+            }
+            if (h == 0) reinterpret_cast<uint16_t*>(op + a.hq * D)[qh * kDt + dt] = f2h(delta);
+        }
+    }
+    }
+    }
+    if (only < 0 || only == t.tok_hi) return;
+    only++;
+    }
+}
+
+// ---- parts joined ----------------------------------------------------------------
+
+// A row's parts in their order, sixteen rows a workgroup: the rows of tiles of
+// M rows that visit their positions in steps of S.
+template <int D, int M, int S>
 __global__ __launch_bounds__(16 * D / 8) void k_paged_join(AttnArgs a)
 {
     int b = blockIdx.x;
     const int head = b % a.hkv;
     b /= a.hkv;
     Tile t;
-    if (!tile_of<16>(a, b / a.row_tiles, (b % a.row_tiles) * 16, t)) return;
-    const Steps<32> steps(t.lo, t.hi, a.window ? a.sink : 0);
+    int sub = 0, req, row0;
+    if (M == 16) {
+        req = b / a.row_tiles;
+        row0 = (b % a.row_tiles) * 16;
+    } else {
+        sub = b % (M / 16);
+        b /= M / 16;
+        req = tile_request(a.row_start, a.n_req, b, a.group, M, a.max_tokens);
+        row0 = (b - first_tile(a.row_start[req], req, a.group, M, a.max_tokens)) * M;
+    }
+    if (row0 < 0 || !tile_of<M>(a, req, row0, t) || (M == 16 ? t.n_rows > a.few : t.n_rows <= a.few)) return;
+    const Steps<S> steps(t.lo, t.hi, a.sink);
     const int parts = min((steps.count + a.part - 1) / a.part, a.splits);
     const int rr = threadIdx.x / (D / 8), c8 = threadIdx.x % (D / 8);
-    if (parts <= 1 || t.row0 + rr >= t.n_rows) return;
-    const int row = t.row0 + rr, tok = t.first_row + row / a.group, qh = head * a.group + row % a.group;
+    const int row = t.row0 + sub * 16 + rr;
+    if (parts <= 1 || row >= t.n_rows) return;
+    const int tok = t.first_row + row / a.group, qh = head * a.group + row % a.group;
     const size_t rows = (size_t)a.max_tokens * a.hq, at = (size_t)tok * a.hq + qh;
-    const float2* ml = reinterpret_cast<const float2*>(a.ws + a.splits * rows * D) + at;
+    const float2* ml = reinterpret_cast<const float2*>(a.ws + a.splits_max * rows * D) + at;
     float top = -__builtin_inff(), total = 0.0f, r[8] = {};
     for (int s = 0; s < parts; s++) top = fmaxf(top, ml[s * rows].x);
     for (int s = 0; s < parts; s++) {
@@ -567,30 +917,71 @@ __global__ __launch_bounds__(16 * D / 8) void k_paged_join(AttnArgs a)
 
 // ---- launches -----------------------------------------------------------------
 
-static void attn_shape(AttnArgs& a, int window, int n_sink)
+// Steps of S positions that a tile of M rows visits at most.
+static long long most_steps(const AttnArgs& a, int M, int S)
 {
-    a.row_tiles = (int)(((long long)min(a.max_new, a.max_tokens) * a.group + 15) / 16);
-    const long long tiles = (long long)a.n_req * a.row_tiles * a.hkv;
-    // steps of a tile at most
-    long long most = ((long long)a.max_kv + 31) / 32;
-    if (window) {
-        const long long seen = (n_sink + 31ll) / 32 + (window + 16ll) / 32 + 2;
+    long long most = ((long long)a.max_kv + S - 1) / S;
+    if (a.window) {
+        const long long seen = (a.sink + S - 1ll) / S + ((long long)a.window + M) / S + 2;
         if (seen < most) most = seen;
     }
-    if (most < 1) most = 1;
-    long long want = tiles > 0 ? (1024 + tiles - 1) / tiles : 1;
-    const long long cap = (most + 3) / 4;  // a step for each wavefront
-    if (want > cap) want = cap;
-    const long long by_len = (most + 31) / 32;  // 1024 positions
-    if (want < by_len && tiles < 65536) want = by_len;
+    return most < 1 ? 1 : most;
+}
+
+static void set_parts(AttnArgs& a, long long most, long long want, int unit)
+{
+    if (want < 1) want = 1;
     if (want > 256) want = 256;
-    a.part = (int)(((most + want - 1) / want + 3) / 4 * 4);
+    a.part = (int)(((most + want - 1) / want + unit - 1) / unit * unit);
     a.splits = (int)((most + a.part - 1) / a.part);
 }
 
-static size_t attn_ws_bytes(const AttnArgs& a, int d)
+// The tiles of sixteen rows, for requests of at most `few` (token, head) rows.
+static void shape16(AttnArgs& a)
 {
-    return a.splits > 1 ? (size_t)a.splits * a.max_tokens * a.hq * (d + 2) * 4 : 0;
+    const long long rows = (long long)(a.max_new < a.max_tokens ? a.max_new : a.max_tokens) * a.group;
+    a.row_tiles = (int)(((rows < a.few ? rows : a.few) + 15) / 16);
+    const long long tiles = (long long)a.n_req * a.row_tiles * a.hkv, most = most_steps(a, 16, 32);
+    long long want = tiles > 0 ? (1024 + tiles - 1) / tiles : 1;
+    if (want > (most + 3) / 4) want = (most + 3) / 4;  // a step for each wavefront
+    const long long by_len = (most + 31) / 32;         // 1024 positions
+    if (want < by_len && tiles < 65536) want = by_len;
+    set_parts(a, most, want, 4);
+}
+
+// The tiles of 128 rows, for the others.
+static void shape_rows(AttnArgs& a, int d)
+{
+    const long long tiles = ((long long)a.max_tokens * a.group / kRowsM + 1) * a.hkv, most = most_steps(a, kRowsM, rows_step(d));
+    long long want = (512 + tiles - 1) / tiles;
+    if (want > (most + 3) / 4) want = (most + 3) / 4;
+    set_parts(a, most, want, 1);
+}
+
+// Rows of a request up to which the sixteen-row tiles take it.
+constexpr int kFewRows = 64;
+
+// One call's launches: each kernel's arguments, those without tiles left out.
+struct AttnPlan {
+    AttnArgs few, rows;
+    bool some_few, some_rows;
+};
+static AttnPlan attn_plan(const AttnArgs& base, int d)
+{
+    AttnPlan p{base, base, true, false};
+    p.few.few = p.rows.few = kFewRows;
+    p.some_rows = (long long)(base.max_new < base.max_tokens ? base.max_new : base.max_tokens) * base.group > kFewRows;
+    shape16(p.few);
+    if (p.some_rows) shape_rows(p.rows, d);
+    const int most = p.some_rows && p.rows.splits > p.few.splits ? p.rows.splits : p.few.splits;
+    p.few.splits_max = p.rows.splits_max = most;
+    return p;
+}
+
+static size_t attn_ws_bytes(const AttnPlan& p, int d)
+{
+    const AttnArgs& a = p.few;
+    return a.splits_max > 1 ? (size_t)a.splits_max * a.max_tokens * a.hq * (d + 2) * 4 : 0;
 }
 
 static int attn_args(AttnArgs& a, const nc_paged_cache* cache, const nc_paged_batch* b, int n_heads, int window,
@@ -621,26 +1012,35 @@ static int attn_args(AttnArgs& a, const nc_paged_cache* cache, const nc_paged_ba
     a.window = window;
     a.sink = window ? (n_sink < a.max_kv ? n_sink : a.max_kv) : 0;
     a.scale = (float)(1.4426950408889634 / sqrt((double)cache->d_head));
-    attn_shape(a, window, a.sink);
     return NC_OK;
 }
 
-template <int D, int CDT>
-static int attn_launch(const AttnArgs& a, hipStream_t st)
+template <int D, int CDT, int QDT>
+static int attn_launch(const AttnPlan& p, hipStream_t st)
 {
-    const long long tiles = (long long)a.n_req * a.row_tiles * a.hkv;
-    NC_CHECK_ARG(tiles * a.splits * 256 <= 0x7FFFFFFFll * 2, "paged_attn: %lld tiles are too many", tiles);
-    const dim3 grid((unsigned)(tiles * a.splits));
-    const bool multi = a.max_new > 1;
-    if (a.q_dtype == F16) {
-        if (multi) hipLaunchKernelGGL((k_paged_attn16<D, CDT, F16, true>), grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((k_paged_attn16<D, CDT, F16, false>), grid, dim3(256), 0, st, a);
-    } else {
-        if (multi) hipLaunchKernelGGL((k_paged_attn16<D, CDT, Q8, true>), grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((k_paged_attn16<D, CDT, Q8, false>), grid, dim3(256), 0, st, a);
+    const AttnArgs &f = p.few, &r = p.rows;
+    const long long tiles = (long long)f.n_req * f.row_tiles * f.hkv;
+    const long long slots = tile_slots(r.max_tokens, r.n_req, r.group, kRowsM) * r.hkv;
+    NC_CHECK_ARG(tiles * f.splits <= 0xFFFFFF && (!p.some_rows || slots * 8 * r.splits <= 0xFFFFFF),
+                 "paged_attn: %lld tiles of %d parts are too many for one launch", tiles > slots ? tiles : slots,
+                 f.splits_max);
+    if (p.some_rows) {
+        hipLaunchKernelGGL((k_paged_rows<D, CDT, QDT>), dim3((unsigned)(slots * r.splits)), dim3(256), 0, st, r);
+        if (r.splits > 1)
+            hipLaunchKernelGGL((k_paged_join<D, kRowsM, rows_step(D)>), dim3((unsigned)(slots * (kRowsM / 16))),
+                               dim3(16 * D / 8), 0, st, r);
     }
-    if (a.splits > 1) hipLaunchKernelGGL((k_paged_join<D>), dim3((unsigned)tiles), dim3(16 * D / 8), 0, st, a);
+    const dim3 grid((unsigned)(tiles * f.splits));
+    hipLaunchKernelGGL((k_paged_attn16<D, CDT, QDT>), grid, dim3(256), 0, st, f);
+    if (f.splits > 1)
+        hipLaunchKernelGGL((k_paged_join<D, 16, 32>), dim3((unsigned)tiles), dim3(16 * D / 8), 0, st, f);
     return launch_status("k_paged_attn16");
+}
+
+template <int D, int CDT>
+static int attn_launch(const AttnPlan& p, hipStream_t st)
+{
+    return p.few.q_dtype == F16 ? attn_launch<D, CDT, F16>(p, st) : attn_launch<D, CDT, Q8>(p, st);
 }
 
 }  // namespace nc
@@ -653,7 +1053,7 @@ extern "C" int nc_paged_attn_workspace(const nc_paged_cache* cache, const nc_pag
     NC_CHECK_ARG(bytes, "paged_attn_workspace: null result");
     AttnArgs a{};
     if (int s = attn_args(a, cache, b, n_heads, window, n_sink)) return s;
-    *bytes = attn_ws_bytes(a, cache->d_head);
+    *bytes = attn_ws_bytes(attn_plan(a, cache->d_head), cache->d_head);
     return NC_OK;
 }
 
@@ -668,7 +1068,7 @@ extern "C" int nc_paged_attn(const nc_tensor* q, const nc_paged_cache* cache, co
                  "paged_attn: q and out are not %d aligned rows of %d values", b->max_tokens, cols);
     NC_CHECK_ARG((q->dtype == NC_F16 || q->dtype == NC_Q8) && (out->dtype == NC_F16 || out->dtype == NC_Q8),
                  "paged_attn: dtypes %d, %d (F16 or Q8)", q->dtype, out->dtype);
-    const size_t need = attn_ws_bytes(a, cache->d_head);
+    const size_t need = attn_ws_bytes(attn_plan(a, cache->d_head), cache->d_head);
     NC_CHECK_ARG(need <= workspace_bytes && (!need || (workspace && aligned16(workspace))),
                  "paged_attn: workspace of %zu bytes (needs %zu, 16-byte aligned)", workspace_bytes, need);
     if (b->max_tokens == 0 || b->max_new == 0 || b->max_kv == 0) return NC_OK;
@@ -680,6 +1080,7 @@ extern "C" int nc_paged_attn(const nc_tensor* q, const nc_paged_cache* cache, co
     a.out_dtype = out->dtype;
     a.ws = (float*)workspace;
     hipStream_t st = stream_of(stream);
-    if (cache->dtype == NC_Q8) return cache->d_head == 64 ? attn_launch<64, Q8>(a, st) : attn_launch<128, Q8>(a, st);
-    return cache->d_head == 64 ? attn_launch<64, F16>(a, st) : attn_launch<128, F16>(a, st);
+    const AttnPlan p = attn_plan(a, cache->d_head);
+    if (cache->dtype == NC_Q8) return cache->d_head == 64 ? attn_launch<64, Q8>(p, st) : attn_launch<128, Q8>(p, st);
+    return cache->d_head == 64 ? attn_launch<64, F16>(p, st) : attn_launch<128, F16>(p, st);
 }
