@@ -58,7 +58,7 @@ __device__ __forceinline__ int tile_request(const int* row_start, int n_req, int
         const int r = lo + lane * step;
         const bool at = lane * step < len && first_tile(row_start[min(r, n_req - 1)], r, per_row, m, max_tokens) <= t;
         const int c = __popcll(__ballot(at));
-        if (c == 0) return lo;  // tables that are no row starts
+        if (c == 0) return __builtin_amdgcn_readfirstlane(lo);  // tables that are no row starts
         lo += (c - 1) * step;
         len = min(step, n_req - lo);
         if (step == 1) return __builtin_amdgcn_readfirstlane(lo);

@@ -109,10 +109,14 @@ struct Seen {
 };
 
 // A page id, or -1 for an entry that is none: callers read page 0 in its
-// place and take its positions for unseen.
+// place and take its positions for unseen.  `pos` is uniform over the
+// wavefront, and the kernels do not write the table: a scalar load, which
+// leaves the vector loads in flight alone.
 __device__ __forceinline__ int page_at(const AttnArgs& a, int req, int pos)
 {
-    const int id = a.table[(size_t)req * a.max_pages + min(pos >> a.lps, a.max_pages - 1)];
+    typedef const __attribute__((address_space(4))) int* ConstInt;
+    const size_t at = (size_t)req * a.max_pages + min(pos >> a.lps, a.max_pages - 1);
+    const int id = reinterpret_cast<ConstInt>(reinterpret_cast<uintptr_t>(a.table))[at];
     return (unsigned)id < (unsigned)a.n_pages ? id : -1;
 }
 
@@ -560,21 +564,25 @@ __device__ __forceinline__ int v_place(int d, int c)
     return d * 2 * rows_step(D) + ((c ^ turn) << 4);
 }
 
-// The pages of a step's sixteens of positions, uniform over a wavefront.
+// The pages of a step's sixteens of positions, uniform over the workgroup
+// (four for steps of 64, two for 32).
 template <int S>
 struct StepPages {
-    int id[S / 16];
-    __device__ __forceinline__ StepPages(const AttnArgs& a, int req, int pos)
+    int a, b, c, d;
+    __device__ __forceinline__ StepPages(const AttnArgs& g, int req, int pos)
     {
-#pragma unroll
-        for (int i = 0; i < S / 16; i++) id[i] = page_at(a, req, pos + 16 * i);
+        a = page_at(g, req, pos);
+        b = page_at(g, req, pos + 16);
+        c = S == 64 ? page_at(g, req, pos + 32) : 0;
+        d = S == 64 ? page_at(g, req, pos + 48) : 0;
     }
-    __device__ __forceinline__ bool all() const
+    __device__ __forceinline__ bool all() const { return (a | b | c | d) >= 0; }
+    __device__ __forceinline__ int at(int i) const
     {
-        bool ok = true;
-#pragma unroll
-        for (int i = 0; i < S / 16; i++) ok &= id[i] >= 0;
-        return ok;
+        // four values first: a choice among members would put them in memory
+        const int w = __builtin_amdgcn_readfirstlane(a), x = __builtin_amdgcn_readfirstlane(b);
+        const int y = __builtin_amdgcn_readfirstlane(c), z = __builtin_amdgcn_readfirstlane(d);
+        return i < 2 ? (i == 0 ? w : x) : (i == 2 ? y : z);
     }
 };
 
@@ -602,10 +610,7 @@ struct KvRows {
                   (a.window && pos <= t.pos0 + t.tok_hi - a.window && pos + kS - 1 >= a.sink);
         // a wavefront's positions lie in one sixteen, whose first row is
         auto row_of = [&](int group) {
-            int id = pages.id[0];
-#pragma unroll
-            for (int i = 1; i < kS / 16; i++) id = group == i ? pages.id[i] : id;
-            return (((size_t)max(id, 0) * a.hkv + head) << a.lps) + ((pos + 16 * group) & mask);
+            return (((size_t)max(pages.at(group), 0) * a.hkv + head) << a.lps) + ((pos + 16 * group) & mask);
         };
 #pragma unroll
         for (int i = 0; i < kNk; i++) {
@@ -621,9 +626,7 @@ struct KvRows {
         }
         const int first = wave * (64 / kDg) * 4, quad = (tid & 63) / kDg;
         const size_t row = row_of(first >> 4);
-        bool page = pages.id[0] >= 0;
-#pragma unroll
-        for (int i = 1; i < kS / 16; i++) page = first >> 4 == i ? pages.id[i] >= 0 : page;
+        const bool page = pages.at(first >> 4) >= 0;
         const uint32_t at = (first & 15) + quad * 4, dg = tid % kDg;
         v_keep = 0;
 #pragma unroll
@@ -702,7 +705,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_paged_rows(AttnArgs a)
     b /= a.hkv;
     const int part = b % a.splits;
     const int slot = b / a.splits;
-    const int req = tile_request(a.row_start, a.n_req, slot, a.group, kRowsM, a.max_tokens);
+    const int req = tile_request(a.row_start, a.n_req, slot, a.group, kRowsM, a.max_tokens);  // uniform
     const int row0 = (slot - first_tile(a.row_start[req], req, a.group, kRowsM, a.max_tokens)) * kRowsM;
     Tile t;
     if (row0 < 0 || !tile_of<kRowsM>(a, req, row0, t) || t.n_rows <= a.few) return;
@@ -767,7 +770,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_paged_rows(AttnArgs a)
 #pragma unroll
                 for (int i = 0; i < 16 * kU; i++) {
                     const int at = (i >> 4) * 32 + ((i >> 2) & 3) * 8 + (i & 3);
-                    const bool seen = (at <= hi) & ((at >= lo) | (at < sk)) & (here.id[at >> 4] >= 0);
+                    const bool seen = (at <= hi) & ((at >= lo) | (at < sk)) & (here.at(at >> 4) >= 0);
                     s[i >> 4][i & 15] = seen ? s[i >> 4][i & 15] : -__builtin_inff();
                 }
             }
