@@ -31,6 +31,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kPScale = 14.0f;  // log2 of the probabilities' scale
+constexpr float kPSlack = 4.0f;   // in 128-row tiles: how far below the maximum its reference point may lie
 
 struct AttnArgs {
     const uint8_t* q;
@@ -50,6 +51,16 @@ struct AttnArgs {
     int splits_max; // of all the call's launches
     float* ws;      // [splits_max][max_tokens * hq][d] sums, then as many (maximum, sum) pairs
 };
+
+// acc + the sum of eight fp16 values, in fp32: a row's weights as they enter
+// the product, so that what their rounding shares cancels in the quotient.
+__device__ __forceinline__ float sum8(half8 v, float acc)
+{
+    const half2v one = {(_Float16)1.0f, (_Float16)1.0f};
+#pragma unroll
+    for (int i = 0; i < 4; i++) acc = __builtin_amdgcn_fdot2(half2v{v[2 * i], v[2 * i + 1]}, one, acc, false);
+    return acc;
+}
 
 // The positions that a tile of rows visits, in steps of S: [0, n_sink) and
 // [lo, hi), as one list of step numbers.
@@ -423,14 +434,9 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 3) void k_paged_attn16(AttnArgs 
         const float base = m_new == -__builtin_inff() ? 0.0f : m_new - kPScale;
         const float alpha = __builtin_amdgcn_exp2f(m - kPScale - base);
         half8 p;
-        float add = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const float e = __builtin_amdgcn_exp2f(x[j] - base);
-            add += e;
-            p[j] = (_Float16)e;
-        }
-        sum = __builtin_fmaf(sum, alpha, add);
+        for (int j = 0; j < 8; j++) p[j] = (_Float16)__builtin_amdgcn_exp2f(x[j] - base);
+        sum = sum8(p, sum * alpha);
         m = m_new;
         if (__ballot(alpha != 1.0f)) {
 #pragma unroll
@@ -586,7 +592,8 @@ struct StepPages {
     }
 };
 
-// One thread's share of a step's K and V, on its way through registers.
+// One thread's share of a step's K and of another step's V, on their way
+// through registers.
 template <int D, int CDT>
 struct KvRows {
     static constexpr int kS = rows_step(D);
@@ -598,24 +605,24 @@ struct KvRows {
     uint16_t kd[CDT == Q8 ? kNk : 1];
     uint2 v[CDT == F16 ? 4 : 1];
     uint32_t vc[CDT == Q8 ? 4 : 1];
-    uint16_t vd[4];
-    uint32_t v_keep;  // a bit for each of the four positions that is to be seen
-    bool partial;     // some of the tile's rows do not see the whole step
+    uint16_t vd[CDT == Q8 ? 4 : 1];
+    int v_pos;    // the first of this thread's four positions
+    bool v_page;  // whether they have a page
+    bool v_part;  // some of the tile's rows do not see the whole step
 
-    __device__ __forceinline__ void load(const AttnArgs& a, const Tile& t, const Seen& see, const StepPages<kS>& pages,
-                                         int head, int pos, int wave)
+    // A wavefront's positions lie in one sixteen of the step; its first row.
+    static __device__ __forceinline__ size_t row_of(const AttnArgs& a, int page, int head, int pos)
     {
-        const int tid = threadIdx.x, mask = (1 << a.lps) - 1;
-        partial = pos + kS - 1 > t.pos0 + t.tok_lo ||
-                  (a.window && pos <= t.pos0 + t.tok_hi - a.window && pos + kS - 1 >= a.sink);
-        // a wavefront's positions lie in one sixteen, whose first row is
-        auto row_of = [&](int group) {
-            return (((size_t)max(pages.at(group), 0) * a.hkv + head) << a.lps) + ((pos + 16 * group) & mask);
-        };
+        return (((size_t)max(page, 0) * a.hkv + head) << a.lps) + (pos & ((1 << a.lps) - 1));
+    }
+
+    __device__ __forceinline__ void load_k(const AttnArgs& a, const StepPages<kS>& pages, int head, int pos, int wave)
+    {
+        const int tid = threadIdx.x;
 #pragma unroll
         for (int i = 0; i < kNk; i++) {
             const int first = i * 2048 / D + wave * 512 / D;  // of the wavefront's positions
-            const size_t row = row_of(first >> 4);
+            const size_t row = row_of(a, pages.at(first >> 4), head, pos + (first & ~15));
             const uint32_t at = (first & 15) + (tid & 63) / (D / 8), c = tid % (D / 8);
             if constexpr (CDT == F16) {
                 k[i] = *reinterpret_cast<const u32x4*>(a.k + row * (2 * D) + (at * D + c * 8) * 2);
@@ -624,15 +631,21 @@ struct KvRows {
                 kd[i] = (a.kd + row * (D / 32))[at * (D / 32) + (c >> 2)];
             }
         }
-        const int first = wave * (64 / kDg) * 4, quad = (tid & 63) / kDg;
-        const size_t row = row_of(first >> 4);
-        const bool page = pages.at(first >> 4) >= 0;
-        const uint32_t at = (first & 15) + quad * 4, dg = tid % kDg;
-        v_keep = 0;
+    }
+
+    __device__ __forceinline__ void load_v(const AttnArgs& a, const Tile& t, const StepPages<kS>& pages, int head, int pos,
+                                           int wave)
+    {
+        const int tid = threadIdx.x;
+        const int first = wave * (64 / kDg) * 4, page = pages.at(first >> 4);
+        const size_t row = row_of(a, page, head, pos + (first & ~15));
+        const uint32_t at = (first & 15) + (tid & 63) / kDg * 4, dg = tid % kDg;
+        v_pos = pos + (first & ~15) + at;
+        v_page = page >= 0;
+        v_part = !v_page || pos + kS - 1 > t.pos0 + t.tok_lo ||
+                 (a.window && pos <= t.pos0 + t.tok_hi - a.window && pos + kS - 1 >= a.sink);
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const int p = pos + first + quad * 4 + j;
-            if (page & (p < see.hi) & ((p >= see.lo) | (p < a.sink))) v_keep |= 1u << j;
             if constexpr (CDT == F16) {
                 v[j] = *reinterpret_cast<const uint2*>(a.v + row * (2 * D) + ((at + j) * D + dg * kE) * 2);
             } else {
@@ -642,9 +655,7 @@ struct KvRows {
         }
     }
 
-    // To shared memory; *not_finite = 1 where rows that see a value that is
-    // no number and rows that do not may meet.
-    __device__ __forceinline__ void store(uint8_t* kb, uint8_t* vb, int* not_finite) const
+    __device__ __forceinline__ void store_k(uint8_t* kb) const
     {
         const int tid = threadIdx.x;
 #pragma unroll
@@ -655,8 +666,14 @@ struct KvRows {
             else w = __builtin_bit_cast(u32x4, dequant8(kc[i], kd[i]).hi);
             *reinterpret_cast<u32x4*>(kb + k_place<D>(key, c)) = w;
         }
+    }
+
+    // Positions that are not to be seen are cleared; *not_finite = 1 where
+    // rows that see a value that is no number and rows that do not may meet.
+    __device__ __forceinline__ void store_v(uint8_t* vb, const AttnArgs& a, const Seen& see, int* not_finite) const
+    {
+        const int tid = threadIdx.x;
         uint2 w[4];
-        bool odd = false;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             if constexpr (CDT == F16) {
@@ -668,16 +685,19 @@ struct KvRows {
                 w[j] = make_uint2(__builtin_bit_cast(uint32_t, x[0] * half2v{d, d}),
                                   __builtin_bit_cast(uint32_t, x[1] * half2v{d, d}));
             }
-            if (partial) {
-                const uint32_t keep = (v_keep >> j) & 1 ? ~0u : 0u;
+        }
+        if (v_part) {
+            bool odd = false;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int p = v_pos + j;
+                const uint32_t keep = v_page & (p < see.hi) & ((p >= see.lo) | (p < a.sink)) ? ~0u : 0u;
                 w[j].x &= keep;
                 w[j].y &= keep;
                 odd |= pair_not_finite(w[j].x) | pair_not_finite(w[j].y);
-            } else if (!((v_keep >> j) & 1)) {
-                w[j] = make_uint2(0, 0);  // no page
             }
+            if (odd) *not_finite = 1;
         }
-        if (odd) *not_finite = 1;
         const int dg = tid % kDg, quad = tid / kDg;  // four positions: the piece and its half
         const int c = (quad >> 2) * 2 + (quad & 1), half = (quad >> 1) & 1;
 #pragma unroll
@@ -692,7 +712,7 @@ struct KvRows {
 };
 
 template <int D, int CDT, int QDT>
-__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_paged_rows(AttnArgs a)
+__global__ __launch_bounds__(256, 2) void k_paged_rows(AttnArgs a)
 {
     constexpr int kS = rows_step(D), kU = kS / 32, kKs = D / 16, kDt = D / 32, kBytes = kS * D * 2;
     __shared__ __align__(16) uint8_t k_sh[2][kBytes];
@@ -741,28 +761,46 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_paged_rows(AttnArgs a)
 #pragma unroll
     for (int i = 0; i < kDt; i++) o[i] = f32x16{};
 
+    // Scores of the step after the one at work are computed beside the
+    // exponentials of the one at work: K runs a step ahead of V.
     KvRows<D, CDT> kv;
-    StepPages<kS> here(a, req, steps.at(v0) * kS), next(a, req, steps.at(min(v0 + 1, v1 - 1)) * kS);
-    kv.load(a, t, see, here, head, steps.at(v0) * kS, wave);
-    kv.store(k_sh[0], v_sh[0], &odd_sh);
+    auto pos_of = [&](int v) { return steps.at(min(v, v1 - 1)) * kS; };
+    half8 kf[kKs][kU];
+    auto read_k = [&](const uint8_t* kb) {
+#pragma unroll
+        for (int ks = 0; ks < kKs; ks++)
+#pragma unroll
+            for (int u = 0; u < kU; u++)
+                kf[ks][u] = *reinterpret_cast<const half8*>(kb + k_place<D>(u * 32 + c, ks * 2 + h));
+    };
+    auto scores = [&](f32x16 (&s)[kU]) {
+#pragma unroll
+        for (int u = 0; u < kU; u++) s[u] = f32x16{};
+#pragma unroll
+        for (int ks = 0; ks < kKs; ks++)
+#pragma unroll
+            for (int u = 0; u < kU; u++) s[u] = mfma32(kf[ks][u], q[ks], s[u]);
+    };
+    StepPages<kS> here(a, req, pos_of(v0)), next(a, req, pos_of(v0 + 1)), after(a, req, pos_of(v0 + 2));
+    kv.load_k(a, here, head, pos_of(v0), wave);
+    kv.load_v(a, t, here, head, pos_of(v0), wave);
+    kv.store_k(k_sh[0]);
+    kv.store_v(v_sh[0], a, see, &odd_sh);
+    kv.load_k(a, next, head, pos_of(v0 + 1), wave);
+    kv.store_k(k_sh[1]);
     __syncthreads();
+    f32x16 s[kU];
+    read_k(k_sh[0]);
+    scores(s);
     for (int v = v0; v < v1; v++) {
         const int buf = (v - v0) & 1, pos = steps.at(v) * kS;
-        if (v + 1 < v1) kv.load(a, t, see, next, head, steps.at(v + 1) * kS, wave);
-        const StepPages<kS> after(a, req, steps.at(min(v + 2, v1 - 1)) * kS);
+        if (v + 2 < v1) kv.load_k(a, after, head, pos_of(v + 2), wave);
+        if (v + 1 < v1) kv.load_v(a, t, next, head, pos_of(v + 1), wave);
+        const StepPages<kS> later(a, req, pos_of(v + 3));
         // unless the wavefront sees none of the step's positions
         if (mine && pos <= t.pos0 + w_hi) {
-            const uint8_t *kb = k_sh[buf], *vb = v_sh[buf];
-            f32x16 s[kU];
-#pragma unroll
-            for (int u = 0; u < kU; u++) s[u] = f32x16{};
-#pragma unroll
-            for (int ks = 0; ks < kKs; ks++)
-#pragma unroll
-                for (int u = 0; u < kU; u++)
-                    s[u] = mfma32(*reinterpret_cast<const half8*>(kb + k_place<D>(u * 32 + c, ks * 2 + h)), q[ks], s[u]);
-            const bool pages = here.all();
-            const bool all = pages & (pos + kS - 1 <= t.pos0 + w_lo) &
+            read_k(k_sh[buf ^ 1]);
+            const bool all = here.all() & (pos + kS - 1 <= t.pos0 + w_lo) &
                              ((a.window == 0) | (pos > t.pos0 + w_hi - a.window) | (pos + kS - 1 < a.sink));
             if (!all) {
                 // against the lane's first position: its others lie at constants
@@ -778,34 +816,57 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_paged_rows(AttnArgs a)
 #pragma unroll
             for (int i = 1; i < 16 * kU; i++) mx = fmaxf(mx, s[i >> 4][i & 15]);
             mx = fmaxf(mx, __shfl_xor(mx, 32)) * a.scale;
-            const float m_new = fmaxf(m, mx);
-            const float base = m_new == -__builtin_inff() ? 0.0f : m_new - kPScale;
-            const float alpha = __builtin_amdgcn_exp2f(m - kPScale - base);
-            half8 p[2 * kU];
-            float add = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 16 * kU; i++) {
-                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 4][i & 15], a.scale, -base));
-                add += e;
-                p[i >> 3][i & 7] = (_Float16)e;
-            }
-            sum = __builtin_fmaf(sum, alpha, add);
-            m = m_new;
-            if (__ballot(alpha != 1.0f)) {
+            // the reference point follows the maximum once it is 2^kPSlack
+            // behind: most steps leave the sums as they are
+            if (__ballot(mx > m + kPSlack)) {
+                const float m_new = fmaxf(m, mx);
+                const float alpha = __builtin_amdgcn_exp2f(m_new == -__builtin_inff() ? 0.0f : m - m_new);
+                sum *= alpha;
 #pragma unroll
                 for (int i = 0; i < kDt; i++) o[i] *= alpha;
+                m = m_new;
+            }
+            const float base = m == -__builtin_inff() ? 0.0f : m - (kPScale - kPSlack);
+            const uint8_t* vb = v_sh[buf];
+            auto read_v = [&](int i) {  // operand i: values 32 (i % kDt) of sixteen i / kDt
+                return *reinterpret_cast<const half8*>(vb + v_place<D>(i % kDt * 32 + c, i / kDt * 2 + h));
+            };
+            constexpr int kNv = 2 * kU * kDt, kAhead = D == 128 ? 4 : 8;
+            half8 vf[kAhead];
+#pragma unroll
+            for (int i = 0; i < kAhead; i++) vf[i] = read_v(i);
+            f32x16 s_next[kU];
+            scores(s_next);
+            half8 p[2 * kU];
+#pragma unroll
+            for (int i = 0; i < 16 * kU; i++)
+                p[i >> 3][i & 7] =
+                    (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 4][i & 15], a.scale, -base));
+            // the reads, then a matrix instruction every few vector ones
+            __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+            for (int i = 0; i < kKs * kU; i++) {
+                __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x2, 40 / kKs, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < kNv; i++) {
+                const half8 f = vf[i % kAhead];
+                if (i + kAhead < kNv) vf[i % kAhead] = read_v(i + kAhead);
+                o[i % kDt] = mfma32(f, p[i / kDt], o[i % kDt]);
+                if (i % kDt == kDt - 1) sum = sum8(p[i / kDt], sum);
             }
 #pragma unroll
-            for (int dt = 0; dt < kDt; dt++)
-#pragma unroll
-                for (int ks = 0; ks < 2 * kU; ks++)
-                    o[dt] = mfma32(*reinterpret_cast<const half8*>(vb + v_place<D>(dt * 32 + c, ks * 2 + h)), p[ks], o[dt]);
+            for (int u = 0; u < kU; u++) s[u] = s_next[u];
         }
-        // the other buffer was last read before the last barrier
-        if (v + 1 < v1) kv.store(k_sh[buf ^ 1], v_sh[buf ^ 1], &odd_sh);
+        // both buffers' last readers are behind the last barrier
+        if (v + 2 < v1) kv.store_k(k_sh[buf]);
+        if (v + 1 < v1) kv.store_v(v_sh[buf ^ 1], a, see, &odd_sh);
         __syncthreads();
         here = next;
         next = after;
+        after = later;
     }
     sum += __shfl_xor(sum, 32);
     if (only < 0 && odd_sh && t.tok_lo != t.tok_hi) {
