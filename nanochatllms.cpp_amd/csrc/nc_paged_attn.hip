@@ -570,25 +570,28 @@ __device__ __forceinline__ int v_place(int d, int c)
     return d * 2 * rows_step(D) + ((c ^ turn) << 4);
 }
 
-// The pages of a step's sixteens of positions, uniform over the workgroup
-// (four for steps of 64, two for 32).
-template <int S>
+// The pages of one step as a wavefront needs them: of the positions whose K
+// and V its threads load, and which sixteens of the step have none (a bit
+// each).  All uniform.
+template <int D>
 struct StepPages {
-    int a, b, c, d;
-    __device__ __forceinline__ StepPages(const AttnArgs& g, int req, int pos)
+    static constexpr int kS = rows_step(D);
+    int k0, k1, v, none;
+    __device__ __forceinline__ StepPages(const AttnArgs& g, int req, int pos, int wave)
     {
-        a = page_at(g, req, pos);
-        b = page_at(g, req, pos + 16);
-        c = S == 64 ? page_at(g, req, pos + 32) : 0;
-        d = S == 64 ? page_at(g, req, pos + 48) : 0;
-    }
-    __device__ __forceinline__ bool all() const { return (a | b | c | d) >= 0; }
-    __device__ __forceinline__ int at(int i) const
-    {
-        // four values first: a choice among members would put them in memory
-        const int w = __builtin_amdgcn_readfirstlane(a), x = __builtin_amdgcn_readfirstlane(b);
-        const int y = __builtin_amdgcn_readfirstlane(c), z = __builtin_amdgcn_readfirstlane(d);
-        return i < 2 ? (i == 0 ? w : x) : (i == 2 ? y : z);
+        const int a = page_at(g, req, pos), b = page_at(g, req, pos + 16);
+        if constexpr (kS == 64) {
+            const int c = page_at(g, req, pos + 32), d = page_at(g, req, pos + 48);
+            k0 = wave < 2 ? a : b;  // positions 8 wave and 32 + 8 wave on
+            k1 = wave < 2 ? c : d;
+            v = wave < 2 ? (wave == 0 ? a : b) : (wave == 2 ? c : d);  // 16 wave on
+            none = (a < 0) | (b < 0) << 1 | (c < 0) << 2 | (d < 0) << 3;
+        } else {
+            k0 = a;  // positions 4 wave and 16 + 4 wave on
+            k1 = b;
+            v = wave < 2 ? a : b;  // 8 wave on
+            none = (a < 0) | (b < 0) << 1;
+        }
     }
 };
 
@@ -616,13 +619,14 @@ struct KvRows {
         return (((size_t)max(page, 0) * a.hkv + head) << a.lps) + (pos & ((1 << a.lps) - 1));
     }
 
-    __device__ __forceinline__ void load_k(const AttnArgs& a, const StepPages<kS>& pages, int head, int pos, int wave)
+    __device__ __forceinline__ void load_k(const AttnArgs& a, int page0, int page1, int head, int pos, int wave)
     {
-        const int tid = threadIdx.x;
+        static_assert(kNk == 2, "two pieces of K a thread");
+        const int tid = threadIdx.x & 255;
 #pragma unroll
         for (int i = 0; i < kNk; i++) {
             const int first = i * 2048 / D + wave * 512 / D;  // of the wavefront's positions
-            const size_t row = row_of(a, pages.at(first >> 4), head, pos + (first & ~15));
+            const size_t row = row_of(a, i == 0 ? page0 : page1, head, pos + (first & ~15));
             const uint32_t at = (first & 15) + (tid & 63) / (D / 8), c = tid % (D / 8);
             if constexpr (CDT == F16) {
                 k[i] = *reinterpret_cast<const u32x4*>(a.k + row * (2 * D) + (at * D + c * 8) * 2);
@@ -633,11 +637,10 @@ struct KvRows {
         }
     }
 
-    __device__ __forceinline__ void load_v(const AttnArgs& a, const Tile& t, const StepPages<kS>& pages, int head, int pos,
-                                           int wave)
+    __device__ __forceinline__ void load_v(const AttnArgs& a, const Tile& t, int page, int head, int pos, int wave)
     {
-        const int tid = threadIdx.x;
-        const int first = wave * (64 / kDg) * 4, page = pages.at(first >> 4);
+        const int tid = threadIdx.x & 255;
+        const int first = wave * (64 / kDg) * 4;
         const size_t row = row_of(a, page, head, pos + (first & ~15));
         const uint32_t at = (first & 15) + (tid & 63) / kDg * 4, dg = tid % kDg;
         v_pos = pos + (first & ~15) + at;
@@ -657,7 +660,7 @@ struct KvRows {
 
     __device__ __forceinline__ void store_k(uint8_t* kb) const
     {
-        const int tid = threadIdx.x;
+        const int tid = threadIdx.x & 255;
 #pragma unroll
         for (int i = 0; i < kNk; i++) {
             const int at = i * 256 + tid, key = at / (D / 8), c = at % (D / 8);
@@ -672,7 +675,7 @@ struct KvRows {
     // rows that see a value that is no number and rows that do not may meet.
     __device__ __forceinline__ void store_v(uint8_t* vb, const AttnArgs& a, const Seen& see, int* not_finite) const
     {
-        const int tid = threadIdx.x;
+        const int tid = threadIdx.x & 255;
         uint2 w[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
@@ -712,13 +715,15 @@ struct KvRows {
 };
 
 template <int D, int CDT, int QDT>
-__global__ __launch_bounds__(256, 2) void k_paged_rows(AttnArgs a)
+__global__ __launch_bounds__(512, 2) void k_paged_rows(AttnArgs a)
 {
     constexpr int kS = rows_step(D), kU = kS / 32, kKs = D / 16, kDt = D / 32, kBytes = kS * D * 2;
-    __shared__ __align__(16) uint8_t k_sh[2][kBytes];
-    __shared__ __align__(16) uint8_t v_sh[2][kBytes];
+    __shared__ __align__(16) uint8_t kv_sh[2][4][kBytes];  // each half's two K and two V buffers
+    __shared__ float2 ml_sh[256];
     __shared__ int odd_sh;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6) & 3, half = __builtin_amdgcn_readfirstlane(tid >> 8);
+    uint8_t (*k_sh)[kBytes] = kv_sh[half], (*v_sh)[kBytes] = kv_sh[half] + 2;
     const int c = lane & 31, h = lane >> 5;
     int b = blockIdx.x;
     const int head = b % a.hkv;
@@ -761,10 +766,13 @@ __global__ __launch_bounds__(256, 2) void k_paged_rows(AttnArgs a)
 #pragma unroll
     for (int i = 0; i < kDt; i++) o[i] = f32x16{};
 
-    // Scores of the step after the one at work are computed beside the
-    // exponentials of the one at work: K runs a step ahead of V.
-    KvRows<D, CDT> kv;
-    auto pos_of = [&](int v) { return steps.at(min(v, v1 - 1)) * kS; };
+    // The halves of the workgroup take turns at the steps.  A half's step i
+    // computes the scores of step i + 1 between the exponentials of step i,
+    // then multiplies those with V of step i; K of step i + 2 and V of step
+    // i + 1 are on their way from memory.
+    const int mine_n = (v1 - v0 - half + 1) / 2, most_n = (v1 - v0 + 1) / 2;
+    auto pos_of = [&](int i) { return steps.at(min(v0 + half + 2 * i, v1 - 1)) * kS; };
+    auto pages_of = [&](int i) { return StepPages<D>(a, req, pos_of(i), wave); };
     half8 kf[kKs][kU];
     auto read_k = [&](const uint8_t* kb) {
 #pragma unroll
@@ -773,34 +781,47 @@ __global__ __launch_bounds__(256, 2) void k_paged_rows(AttnArgs a)
             for (int u = 0; u < kU; u++)
                 kf[ks][u] = *reinterpret_cast<const half8*>(kb + k_place<D>(u * 32 + c, ks * 2 + h));
     };
-    auto scores = [&](f32x16 (&s)[kU]) {
-#pragma unroll
-        for (int u = 0; u < kU; u++) s[u] = f32x16{};
-#pragma unroll
-        for (int ks = 0; ks < kKs; ks++)
-#pragma unroll
-            for (int u = 0; u < kU; u++) s[u] = mfma32(kf[ks][u], q[ks], s[u]);
-    };
-    StepPages<kS> here(a, req, pos_of(v0)), next(a, req, pos_of(v0 + 1)), after(a, req, pos_of(v0 + 2));
-    kv.load_k(a, here, head, pos_of(v0), wave);
-    kv.load_v(a, t, here, head, pos_of(v0), wave);
-    kv.store_k(k_sh[0]);
-    kv.store_v(v_sh[0], a, see, &odd_sh);
-    kv.load_k(a, next, head, pos_of(v0 + 1), wave);
-    kv.store_k(k_sh[1]);
+    KvRows<D, CDT> kv;
+    f32x16 s[kU], t_s[kU];
+    int v_page, none;  // V's page of the next step; four bits for each of three steps from this one
+    StepPages<D> later = pages_of(2);
+    {
+        const StepPages<D> p0 = pages_of(0), p1 = pages_of(1);
+        KvRows<D, CDT> w;
+        kv.load_k(a, p0.k0, p0.k1, head, pos_of(0), wave);
+        kv.load_v(a, t, p0.v, head, pos_of(0), wave);
+        w.load_k(a, p1.k0, p1.k1, head, pos_of(1), wave);
+        kv.store_k(k_sh[0]);
+        kv.store_v(v_sh[0], a, see, &odd_sh);
+        w.store_k(k_sh[1]);
+        v_page = p1.v;
+        none = p0.none | p1.none << 4;
+    }
     __syncthreads();
-    f32x16 s[kU];
     read_k(k_sh[0]);
-    scores(s);
-    for (int v = v0; v < v1; v++) {
-        const int buf = (v - v0) & 1, pos = steps.at(v) * kS;
-        if (v + 2 < v1) kv.load_k(a, after, head, pos_of(v + 2), wave);
-        if (v + 1 < v1) kv.load_v(a, t, next, head, pos_of(v + 1), wave);
-        const StepPages<kS> later(a, req, pos_of(v + 3));
+#pragma unroll
+    for (int u = 0; u < kU; u++) s[u] = t_s[u] = f32x16{};
+#pragma unroll
+    for (int ks = 0; ks < kKs; ks++)
+#pragma unroll
+        for (int u = 0; u < kU; u++) s[u] = mfma32(kf[ks][u], q[ks], s[u]);
+    __syncthreads();
+    auto step = [&](f32x16 (&s)[kU], f32x16 (&s_next)[kU], int i0, int buf) {
+        const int pos = pos_of(i0);
+        if (i0 + 2 < mine_n) kv.load_k(a, later.k0, later.k1, head, pos_of(i0 + 2), wave);
+        if (i0 + 1 < mine_n) kv.load_v(a, t, v_page, head, pos_of(i0 + 1), wave);
+        v_page = later.v;
+        none |= later.none << 8;
+        const StepPages<D> far = pages_of(i0 + 3);
         // unless the wavefront sees none of the step's positions
-        if (mine && pos <= t.pos0 + w_hi) {
+        if (mine && i0 < mine_n && pos <= t.pos0 + w_hi) {
+            const uint8_t* vb = v_sh[buf];
+            auto read_v = [&](int i) {  // operand i: values 32 (i % kDt) of sixteen i / kDt
+                return *reinterpret_cast<const half8*>(vb + v_place<D>(i % kDt * 32 + c, i / kDt * 2 + h));
+            };
+            constexpr int kNv = 2 * kU * kDt, kAhead = D == 128 ? 4 : 8;
             read_k(k_sh[buf ^ 1]);
-            const bool all = here.all() & (pos + kS - 1 <= t.pos0 + w_lo) &
+            const bool all = ((none & 15) == 0) & (pos + kS - 1 <= t.pos0 + w_lo) &
                              ((a.window == 0) | (pos > t.pos0 + w_hi - a.window) | (pos + kS - 1 < a.sink));
             if (!all) {
                 // against the lane's first position: its others lie at constants
@@ -808,7 +829,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_rows(AttnArgs a)
 #pragma unroll
                 for (int i = 0; i < 16 * kU; i++) {
                     const int at = (i >> 4) * 32 + ((i >> 2) & 3) * 8 + (i & 3);
-                    const bool seen = (at <= hi) & ((at >= lo) | (at < sk)) & (here.at(at >> 4) >= 0);
+                    const bool seen = (at <= hi) & ((at >= lo) | (at < sk)) & !((none >> (at >> 4)) & 1);
                     s[i >> 4][i & 15] = seen ? s[i >> 4][i & 15] : -__builtin_inff();
                 }
             }
@@ -827,53 +848,82 @@ __global__ __launch_bounds__(256, 2) void k_paged_rows(AttnArgs a)
                 m = m_new;
             }
             const float base = m == -__builtin_inff() ? 0.0f : m - (kPScale - kPSlack);
-            const uint8_t* vb = v_sh[buf];
-            auto read_v = [&](int i) {  // operand i: values 32 (i % kDt) of sixteen i / kDt
-                return *reinterpret_cast<const half8*>(vb + v_place<D>(i % kDt * 32 + c, i / kDt * 2 + h));
-            };
-            constexpr int kNv = 2 * kU * kDt, kAhead = D == 128 ? 4 : 8;
-            half8 vf[kAhead];
+            // Each matrix instruction of the next step's scores between some
+            // of this step's exponentials: in a run of their own each kind
+            // leaves the other's unit idle, in step with the other wavefronts.
+            half8 p[2 * kU], vf[kAhead];
 #pragma unroll
             for (int i = 0; i < kAhead; i++) vf[i] = read_v(i);
-            f32x16 s_next[kU];
-            scores(s_next);
-            half8 p[2 * kU];
+            constexpr int kN = kKs * kU, kEach = 16 * kU / kN;
 #pragma unroll
-            for (int i = 0; i < 16 * kU; i++)
-                p[i >> 3][i & 7] =
-                    (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 4][i & 15], a.scale, -base));
-            // the reads, then a matrix instruction every few vector ones
-            __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+            for (int u = 0; u < kU; u++) s_next[u] = f32x16{};
 #pragma unroll
-            for (int i = 0; i < kKs * kU; i++) {
-                __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x2, 40 / kKs, 0);
+            for (int n = 0; n < kN; n++) {
+                s_next[n % kU] = mfma32(kf[n / kU][n % kU], q[n / kU], s_next[n % kU]);
+#pragma unroll
+                for (int i = n * kEach; i < (n + 1) * kEach; i++)
+                    p[i >> 3][i & 7] =
+                        (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 4][i & 15], a.scale, -base));
+                __builtin_amdgcn_sched_barrier(0);
             }
-            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int i = 0; i < kNv; i++) {
                 const half8 f = vf[i % kAhead];
                 if (i + kAhead < kNv) vf[i % kAhead] = read_v(i + kAhead);
                 o[i % kDt] = mfma32(f, p[i / kDt], o[i % kDt]);
                 if (i % kDt == kDt - 1) sum = sum8(p[i / kDt], sum);
+                __builtin_amdgcn_sched_barrier(0);
             }
-#pragma unroll
-            for (int u = 0; u < kU; u++) s[u] = s_next[u];
         }
-        // both buffers' last readers are behind the last barrier
-        if (v + 2 < v1) kv.store_k(k_sh[buf]);
-        if (v + 1 < v1) kv.store_v(v_sh[buf ^ 1], a, see, &odd_sh);
+        // what these overwrite was last read before the last barrier
+        if (i0 + 2 < mine_n) kv.store_k(k_sh[buf]);
+        if (i0 + 1 < mine_n) kv.store_v(v_sh[buf ^ 1], a, see, &odd_sh);
         __syncthreads();
-        here = next;
-        next = after;
-        after = later;
+        none >>= 4;
+        later = far;
+    };
+    for (int i0 = 0; i0 < most_n; i0 += 2) {
+        step(s, t_s, i0, 0);
+        if (i0 + 1 < most_n) step(t_s, s, i0 + 1, 1);
     }
     sum += __shfl_xor(sum, 32);
     if (only < 0 && odd_sh && t.tok_lo != t.tok_hi) {
         only = t.tok_lo;
+        __syncthreads();  // odd_sh is read before it is written again
         continue;
     }
-    if (first + c < t.n_rows && (only < 0 || only == my_tok)) {
+    // the second half's sums to the first, through the buffers
+    float4* const o_sh = reinterpret_cast<float4*>(&kv_sh[0][0][0]) + (wave * 64 + lane);
+    static_assert(256 * kDt * 64 <= sizeof(kv_sh), "the sums fit the buffers");
+    if (half == 1) {
+#pragma unroll
+        for (int dt = 0; dt < kDt; dt++)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                o_sh[(dt * 4 + j) * 256] =
+                    make_float4(o[dt][4 * j], o[dt][4 * j + 1], o[dt][4 * j + 2], o[dt][4 * j + 3]);
+        ml_sh[wave * 64 + lane] = make_float2(m, sum);
+    }
+    __syncthreads();
+    if (half == 0) {
+        const float2 e = ml_sh[wave * 64 + lane];
+        const float top = fmaxf(m, e.x);
+        const float f0 = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+        const float f1 = e.x == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(e.x - top);
+        m = top;
+        sum = sum * f0 + e.y * f1;
+#pragma unroll
+        for (int dt = 0; dt < kDt; dt++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float4 w = o_sh[(dt * 4 + j) * 256];
+                o[dt][4 * j] = o[dt][4 * j] * f0 + w.x * f1;
+                o[dt][4 * j + 1] = o[dt][4 * j + 1] * f0 + w.y * f1;
+                o[dt][4 * j + 2] = o[dt][4 * j + 2] * f0 + w.z * f1;
+                o[dt][4 * j + 3] = o[dt][4 * j + 3] * f0 + w.w * f1;
+            }
+    }
+    if (half == 0 && first + c < t.n_rows && (only < 0 || only == my_tok)) {
 
     // lane (c, h): row c, values 32 dt + 8 j + 4 h + i
     const int tok = t.first_row + my_tok, qh = head * a.group + my % a.group;
@@ -923,6 +973,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_rows(AttnArgs a)
     }
     if (only < 0 || only == t.tok_hi) return;
     only++;
+    __syncthreads();  // the sums are read before the buffers are written again
     }
 }
 
@@ -1089,7 +1140,7 @@ static int attn_launch(const AttnPlan& p, hipStream_t st)
                  "paged_attn: %lld tiles of %d parts are too many for one launch", tiles > slots ? tiles : slots,
                  f.splits_max);
     if (p.some_rows) {
-        hipLaunchKernelGGL((k_paged_rows<D, CDT, QDT>), dim3((unsigned)(slots * r.splits)), dim3(256), 0, st, r);
+        hipLaunchKernelGGL((k_paged_rows<D, CDT, QDT>), dim3((unsigned)(slots * r.splits)), dim3(512), 0, st, r);
         if (r.splits > 1)
             hipLaunchKernelGGL((k_paged_join<D, kRowsM, rows_step(D)>), dim3((unsigned)(slots * (kRowsM / 16))),
                                dim3(16 * D / 8), 0, st, r);
