@@ -324,16 +324,23 @@ __device__ __forceinline__ half8 v_operand(const uint32_t (&w)[8], bool odd)
     return __builtin_bit_cast(half8, o);
 }
 
+template <int D>
+struct Shared16 {
+    float o[4][16][D + 4];
+    float ml[4][16][2];
+    int odd;
+};
+
+// Workgroup b of the sixteen-row tiles.
 template <int D, int CDT, int QDT>
-__global__ __launch_bounds__(256, D == 64 ? 4 : 3) void k_paged_attn16(AttnArgs a)
+__device__ __forceinline__ void attn16(const AttnArgs& a, int b, Shared16<D>& sh)
 {
-    constexpr int kKs = D / 32, kDt = D / 16, kPitch = D + 4;
-    __shared__ float o_sh[4][16][kPitch];
-    __shared__ float ml_sh[4][16][2];
-    __shared__ int odd_sh;
+    constexpr int kKs = D / 32, kDt = D / 16;
+    auto& o_sh = sh.o;
+    auto& ml_sh = sh.ml;
+    int& odd_sh = sh.odd;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 15, g = lane >> 4;
-    int b = blockIdx.x;
     const int part = b % a.splits;
     b /= a.splits;
     const int head = b % a.hkv;
@@ -530,6 +537,13 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 3) void k_paged_attn16(AttnArgs 
     }
 }
 
+template <int D, int CDT, int QDT>
+__global__ __launch_bounds__(256, D == 64 ? 4 : 3) void k_paged_attn16(AttnArgs a)
+{
+    __shared__ Shared16<D> sh;
+    attn16<D, CDT, QDT>(a, blockIdx.x, sh);
+}
+
 // ---- 128 rows a tile -----------------------------------------------------------
 //
 // One workgroup of four wavefronts per (tile, kv head, part of the
@@ -570,29 +584,15 @@ __device__ __forceinline__ int v_place(int d, int c)
     return d * 2 * rows_step(D) + ((c ^ turn) << 4);
 }
 
-// The pages of one step as a wavefront needs them: of the positions whose K
-// and V its threads load, and which sixteens of the step have none (a bit
-// each).  All uniform.
-template <int D>
-struct StepPages {
-    static constexpr int kS = rows_step(D);
-    int k0, k1, v, none;
-    __device__ __forceinline__ StepPages(const AttnArgs& g, int req, int pos, int wave)
-    {
-        const int a = page_at(g, req, pos), b = page_at(g, req, pos + 16);
-        if constexpr (kS == 64) {
-            const int c = page_at(g, req, pos + 32), d = page_at(g, req, pos + 48);
-            k0 = wave < 2 ? a : b;  // positions 8 wave and 32 + 8 wave on
-            k1 = wave < 2 ? c : d;
-            v = wave < 2 ? (wave == 0 ? a : b) : (wave == 2 ? c : d);  // 16 wave on
-            none = (a < 0) | (b < 0) << 1 | (c < 0) << 2 | (d < 0) << 3;
-        } else {
-            k0 = a;  // positions 4 wave and 16 + 4 wave on
-            k1 = b;
-            v = wave < 2 ? a : b;  // 8 wave on
-            none = (a < 0) | (b < 0) << 1;
-        }
-    }
+// Where the pages lie: the byte offset of the first row of every sixteen
+// positions of up to kPlaces / (sixteens of a step) steps, looked up once for
+// the workgroup.  A lookup for every step, by every wavefront, took a fifth
+// of its instructions.
+constexpr int kPlaces = 1024;
+struct Places {
+    unsigned long long at[kPlaces];
+    uint32_t none[kPlaces / 32];  // a bit for each sixteen without a page
+    int some_none;
 };
 
 // One thread's share of a step's K and of another step's V, on their way
@@ -609,58 +609,50 @@ struct KvRows {
     uint2 v[CDT == F16 ? 4 : 1];
     uint32_t vc[CDT == Q8 ? 4 : 1];
     uint16_t vd[CDT == Q8 ? 4 : 1];
-    int v_pos;    // the first of this thread's four positions
-    bool v_page;  // whether they have a page
-    bool v_part;  // some of the tile's rows do not see the whole step
+    // A wavefront's positions lie in one sixteen of the step.
+    static __device__ __forceinline__ int k_sixteen(int i, int wave) { return (i * 2048 / D + wave * 512 / D) >> 4; }
+    static __device__ __forceinline__ int v_sixteen(int wave) { return (wave * (64 / kDg) * 4) >> 4; }
 
-    // A wavefront's positions lie in one sixteen of the step; its first row.
-    static __device__ __forceinline__ size_t row_of(const AttnArgs& a, int page, int head, int pos)
-    {
-        return (((size_t)max(page, 0) * a.hkv + head) << a.lps) + (pos & ((1 << a.lps) - 1));
-    }
-
-    __device__ __forceinline__ void load_k(const AttnArgs& a, int page0, int page1, int head, int pos, int wave)
+    // at0, at1: the places of the wavefront's sixteens.
+    __device__ __forceinline__ void load_k(const AttnArgs& a, unsigned long long at0, unsigned long long at1, int wave)
     {
         static_assert(kNk == 2, "two pieces of K a thread");
-        const int tid = threadIdx.x & 255;
+        const int tid = threadIdx.x;
 #pragma unroll
         for (int i = 0; i < kNk; i++) {
             const int first = i * 2048 / D + wave * 512 / D;  // of the wavefront's positions
-            const size_t row = row_of(a, i == 0 ? page0 : page1, head, pos + (first & ~15));
-            const uint32_t at = (first & 15) + (tid & 63) / (D / 8), c = tid % (D / 8);
+            const unsigned long long at = i == 0 ? at0 : at1;
+            const uint32_t key = (first & 15) + (tid & 63) / (D / 8), c = tid % (D / 8);
             if constexpr (CDT == F16) {
-                k[i] = *reinterpret_cast<const u32x4*>(a.k + row * (2 * D) + (at * D + c * 8) * 2);
+                k[i] = *reinterpret_cast<const u32x4*>(a.k + at + (key * D + c * 8) * 2);
             } else {
-                kc[i] = *reinterpret_cast<const uint2*>(a.k + row * D + (at * D + c * 8));
-                kd[i] = (a.kd + row * (D / 32))[at * (D / 32) + (c >> 2)];
+                kc[i] = *reinterpret_cast<const uint2*>(a.k + at + (key * D + c * 8));
+                kd[i] = *(reinterpret_cast<const uint16_t*>(reinterpret_cast<const uint8_t*>(a.kd) + (at >> 4)) +
+                          (key * (D / 32) + (c >> 2)));
             }
         }
     }
 
-    __device__ __forceinline__ void load_v(const AttnArgs& a, const Tile& t, int page, int head, int pos, int wave)
+    __device__ __forceinline__ void load_v(const AttnArgs& a, unsigned long long at, int wave)
     {
-        const int tid = threadIdx.x & 255;
+        const int tid = threadIdx.x;
         const int first = wave * (64 / kDg) * 4;
-        const size_t row = row_of(a, page, head, pos + (first & ~15));
-        const uint32_t at = (first & 15) + (tid & 63) / kDg * 4, dg = tid % kDg;
-        v_pos = pos + (first & ~15) + at;
-        v_page = page >= 0;
-        v_part = !v_page || pos + kS - 1 > t.pos0 + t.tok_lo ||
-                 (a.window && pos <= t.pos0 + t.tok_hi - a.window && pos + kS - 1 >= a.sink);
+        const uint32_t key = (first & 15) + (tid & 63) / kDg * 4, dg = tid % kDg;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             if constexpr (CDT == F16) {
-                v[j] = *reinterpret_cast<const uint2*>(a.v + row * (2 * D) + ((at + j) * D + dg * kE) * 2);
+                v[j] = *reinterpret_cast<const uint2*>(a.v + at + ((key + j) * D + dg * kE) * 2);
             } else {
-                vc[j] = *reinterpret_cast<const uint32_t*>(a.v + row * D + ((at + j) * D + dg * kE));
-                vd[j] = (a.vd + row * (D / 32))[(at + j) * (D / 32) + dg * kE / 32];
+                vc[j] = *reinterpret_cast<const uint32_t*>(a.v + at + ((key + j) * D + dg * kE));
+                vd[j] = *(reinterpret_cast<const uint16_t*>(reinterpret_cast<const uint8_t*>(a.vd) + (at >> 4)) +
+                          ((key + j) * (D / 32) + dg * kE / 32));
             }
         }
     }
 
     __device__ __forceinline__ void store_k(uint8_t* kb) const
     {
-        const int tid = threadIdx.x & 255;
+        const int tid = threadIdx.x;
 #pragma unroll
         for (int i = 0; i < kNk; i++) {
             const int at = i * 256 + tid, key = at / (D / 8), c = at % (D / 8);
@@ -673,9 +665,11 @@ struct KvRows {
 
     // Positions that are not to be seen are cleared; *not_finite = 1 where
     // rows that see a value that is no number and rows that do not may meet.
-    __device__ __forceinline__ void store_v(uint8_t* vb, const AttnArgs& a, const Seen& see, int* not_finite) const
+    // `part`: some of the tile's rows do not see all of the step at pos.
+    __device__ __forceinline__ void store_v(uint8_t* vb, const AttnArgs& a, const Seen& see, bool part, int pos,
+                                            bool page, int* not_finite) const
     {
-        const int tid = threadIdx.x & 255;
+        const int tid = threadIdx.x;
         uint2 w[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
@@ -689,12 +683,12 @@ struct KvRows {
                                   __builtin_bit_cast(uint32_t, x[1] * half2v{d, d}));
             }
         }
-        if (v_part) {
+        if (part) {
             bool odd = false;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const int p = v_pos + j;
-                const uint32_t keep = v_page & (p < see.hi) & ((p >= see.lo) | (p < a.sink)) ? ~0u : 0u;
+                const int p = pos + tid / kDg * 4 + j;
+                const uint32_t keep = page & (p < see.hi) & ((p >= see.lo) | (p < a.sink)) ? ~0u : 0u;
                 w[j].x &= keep;
                 w[j].y &= keep;
                 odd |= pair_not_finite(w[j].x) | pair_not_finite(w[j].y);
@@ -714,18 +708,24 @@ struct KvRows {
     }
 };
 
+template <int D>
+struct SharedRows {
+    uint8_t kv[4][rows_step(D) * D * 2];  // two K and two V buffers
+    Places places;
+    int odd;
+};
+
+// Workgroup b of the 128-row tiles.
 template <int D, int CDT, int QDT>
-__global__ __launch_bounds__(512, 2) void k_paged_rows(AttnArgs a)
+__device__ __forceinline__ void attn_rows(const AttnArgs& a, int b, SharedRows<D>& sh)
 {
-    constexpr int kS = rows_step(D), kU = kS / 32, kKs = D / 16, kDt = D / 32, kBytes = kS * D * 2;
-    __shared__ __align__(16) uint8_t kv_sh[2][4][kBytes];  // each half's two K and two V buffers
-    __shared__ float2 ml_sh[256];
-    __shared__ int odd_sh;
+    constexpr int kS = rows_step(D), kG = kS / 16, kU = kS / 32, kKs = D / 16, kDt = D / 32, kBytes = kS * D * 2;
+    Places& places = sh.places;
+    int& odd_sh = sh.odd;
     const int tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6) & 3, half = __builtin_amdgcn_readfirstlane(tid >> 8);
-    uint8_t (*k_sh)[kBytes] = kv_sh[half], (*v_sh)[kBytes] = kv_sh[half] + 2;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    uint8_t (*k_sh)[kBytes] = sh.kv, (*v_sh)[kBytes] = sh.kv + 2;
     const int c = lane & 31, h = lane >> 5;
-    int b = blockIdx.x;
     const int head = b % a.hkv;
     b /= a.hkv;
     const int part = b % a.splits;
@@ -766,13 +766,32 @@ __global__ __launch_bounds__(512, 2) void k_paged_rows(AttnArgs a)
 #pragma unroll
     for (int i = 0; i < kDt; i++) o[i] = f32x16{};
 
-    // The halves of the workgroup take turns at the steps.  A half's step i
-    // computes the scores of step i + 1 between the exponentials of step i,
-    // then multiplies those with V of step i; K of step i + 2 and V of step
-    // i + 1 are on their way from memory.
-    const int mine_n = (v1 - v0 - half + 1) / 2, most_n = (v1 - v0 + 1) / 2;
-    auto pos_of = [&](int i) { return steps.at(min(v0 + half + 2 * i, v1 - 1)) * kS; };
-    auto pages_of = [&](int i) { return StepPages<D>(a, req, pos_of(i), wave); };
+    for (int vt = v0; vt < v1; vt += kPlaces / kG) {
+    const int vn = min(v1 - vt, kPlaces / kG);
+    if (vt != v0) __syncthreads();  // the places are read before they are written again
+    if (tid < kPlaces / 32) places.none[tid] = 0;
+    if (tid == 0) places.some_none = 0;
+    __syncthreads();
+    for (int e = tid; e < vn * kG; e += 256) {
+        const int pos = steps.at(vt + e / kG) * kS + e % kG * 16;
+        const int id = a.table[(size_t)req * a.max_pages + min(pos >> a.lps, a.max_pages - 1)];
+        const bool page = (unsigned)id < (unsigned)a.n_pages;
+        const size_t row = (((size_t)(page ? id : 0) * a.hkv + head) << a.lps) + (pos & ((1 << a.lps) - 1));
+        places.at[e] = row * (CDT == Q8 ? D : 2 * D);
+        // sixteens that no row sees are masked by their positions
+        if (!page && pos < t.hi && (pos + 15 >= t.lo || pos < a.sink)) {
+            atomicOr(&places.none[e >> 5], 1u << (e & 31));
+            places.some_none = 1;
+        }
+    }
+    __syncthreads();
+    const bool some_none = places.some_none != 0;
+
+    // Step i computes the scores of step i + 1 between its exponentials, then
+    // multiplies those with its V; K of step i + 2 and V of step i + 1 are on
+    // their way from memory.
+    auto clamped = [&](int i) { return min(i, vn - 1); };
+    auto pos_of = [&](int i) { return steps.at(vt + clamped(i)) * kS; };
     half8 kf[kKs][kU];
     auto read_k = [&](const uint8_t* kb) {
 #pragma unroll
@@ -781,21 +800,37 @@ __global__ __launch_bounds__(512, 2) void k_paged_rows(AttnArgs a)
             for (int u = 0; u < kU; u++)
                 kf[ks][u] = *reinterpret_cast<const half8*>(kb + k_place<D>(u * 32 + c, ks * 2 + h));
     };
+    // whether all rows from token lo to hi see the whole step at pos
+    auto all_see = [&](int pos, int lo, int hi) {
+        return !some_none & (pos + kS - 1 <= t.pos0 + lo) &
+               ((a.window == 0) | (pos > t.pos0 + hi - a.window) | (pos + kS - 1 < a.sink));
+    };
+    // places of the next loads, read a step ahead
+    unsigned long long k_at0, k_at1, v_at;
+    auto places_of = [&](int ik, int iv) {
+        const unsigned long long* p = places.at + clamped(ik) * kG;
+        k_at0 = p[KvRows<D, CDT>::k_sixteen(0, wave)];
+        k_at1 = p[KvRows<D, CDT>::k_sixteen(1, wave)];
+        v_at = places.at[clamped(iv) * kG + KvRows<D, CDT>::v_sixteen(wave)];
+    };
+    auto store_v = [&](const KvRows<D, CDT>& from, uint8_t* vb, int i) {
+        const int pos = pos_of(i), e = clamped(i) * kG + KvRows<D, CDT>::v_sixteen(wave);
+        const bool page = !some_none || !((places.none[e >> 5] >> (e & 31)) & 1);
+        from.store_v(vb, a, see, !all_see(pos, t.tok_lo, t.tok_hi), pos, page, &odd_sh);
+    };
     KvRows<D, CDT> kv;
     f32x16 s[kU], t_s[kU];
-    int v_page, none;  // V's page of the next step; four bits for each of three steps from this one
-    StepPages<D> later = pages_of(2);
     {
-        const StepPages<D> p0 = pages_of(0), p1 = pages_of(1);
         KvRows<D, CDT> w;
-        kv.load_k(a, p0.k0, p0.k1, head, pos_of(0), wave);
-        kv.load_v(a, t, p0.v, head, pos_of(0), wave);
-        w.load_k(a, p1.k0, p1.k1, head, pos_of(1), wave);
+        places_of(0, 0);
+        kv.load_k(a, k_at0, k_at1, wave);
+        kv.load_v(a, v_at, wave);
+        places_of(1, 1);
+        w.load_k(a, k_at0, k_at1, wave);
+        places_of(2, 1);
         kv.store_k(k_sh[0]);
-        kv.store_v(v_sh[0], a, see, &odd_sh);
+        store_v(kv, v_sh[0], 0);
         w.store_k(k_sh[1]);
-        v_page = p1.v;
-        none = p0.none | p1.none << 4;
     }
     __syncthreads();
     read_k(k_sh[0]);
@@ -807,25 +842,23 @@ __global__ __launch_bounds__(512, 2) void k_paged_rows(AttnArgs a)
         for (int u = 0; u < kU; u++) s[u] = mfma32(kf[ks][u], q[ks], s[u]);
     __syncthreads();
     auto step = [&](f32x16 (&s)[kU], f32x16 (&s_next)[kU], int i0, int buf) {
+        if (i0 + 2 < vn) kv.load_k(a, k_at0, k_at1, wave);
+        if (i0 + 1 < vn) kv.load_v(a, v_at, wave);
+        places_of(i0 + 3, i0 + 2);
         const int pos = pos_of(i0);
-        if (i0 + 2 < mine_n) kv.load_k(a, later.k0, later.k1, head, pos_of(i0 + 2), wave);
-        if (i0 + 1 < mine_n) kv.load_v(a, t, v_page, head, pos_of(i0 + 1), wave);
-        v_page = later.v;
-        none |= later.none << 8;
-        const StepPages<D> far = pages_of(i0 + 3);
         // unless the wavefront sees none of the step's positions
-        if (mine && i0 < mine_n && pos <= t.pos0 + w_hi) {
+        if (mine && pos <= t.pos0 + w_hi) {
             const uint8_t* vb = v_sh[buf];
             auto read_v = [&](int i) {  // operand i: values 32 (i % kDt) of sixteen i / kDt
                 return *reinterpret_cast<const half8*>(vb + v_place<D>(i % kDt * 32 + c, i / kDt * 2 + h));
             };
             constexpr int kNv = 2 * kU * kDt, kAhead = D == 128 ? 4 : 8;
             read_k(k_sh[buf ^ 1]);
-            const bool all = ((none & 15) == 0) & (pos + kS - 1 <= t.pos0 + w_lo) &
-                             ((a.window == 0) | (pos > t.pos0 + w_hi - a.window) | (pos + kS - 1 < a.sink));
-            if (!all) {
+            if (!all_see(pos, w_lo, w_hi)) {
                 // against the lane's first position: its others lie at constants
                 const int at0 = pos + 4 * h, hi = my_pos - at0, lo = my_lo - at0, sk = a.sink - at0;
+                int none = 0;
+                if (some_none) none = places.none[clamped(i0) * kG >> 5] >> (clamped(i0) * kG & 31);
 #pragma unroll
                 for (int i = 0; i < 16 * kU; i++) {
                     const int at = (i >> 4) * 32 + ((i >> 2) & 3) * 8 + (i & 3);
@@ -876,15 +909,14 @@ __global__ __launch_bounds__(512, 2) void k_paged_rows(AttnArgs a)
             }
         }
         // what these overwrite was last read before the last barrier
-        if (i0 + 2 < mine_n) kv.store_k(k_sh[buf]);
-        if (i0 + 1 < mine_n) kv.store_v(v_sh[buf ^ 1], a, see, &odd_sh);
+        if (i0 + 2 < vn) kv.store_k(k_sh[buf]);
+        if (i0 + 1 < vn) store_v(kv, v_sh[buf ^ 1], i0 + 1);
         __syncthreads();
-        none >>= 4;
-        later = far;
     };
-    for (int i0 = 0; i0 < most_n; i0 += 2) {
+    for (int i0 = 0; i0 < vn; i0 += 2) {
         step(s, t_s, i0, 0);
-        if (i0 + 1 < most_n) step(t_s, s, i0 + 1, 1);
+        if (i0 + 1 < vn) step(t_s, s, i0 + 1, 1);
+    }
     }
     sum += __shfl_xor(sum, 32);
     if (only < 0 && odd_sh && t.tok_lo != t.tok_hi) {
@@ -892,38 +924,7 @@ __global__ __launch_bounds__(512, 2) void k_paged_rows(AttnArgs a)
         __syncthreads();  // odd_sh is read before it is written again
         continue;
     }
-    // the second half's sums to the first, through the buffers
-    float4* const o_sh = reinterpret_cast<float4*>(&kv_sh[0][0][0]) + (wave * 64 + lane);
-    static_assert(256 * kDt * 64 <= sizeof(kv_sh), "the sums fit the buffers");
-    if (half == 1) {
-#pragma unroll
-        for (int dt = 0; dt < kDt; dt++)
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-                o_sh[(dt * 4 + j) * 256] =
-                    make_float4(o[dt][4 * j], o[dt][4 * j + 1], o[dt][4 * j + 2], o[dt][4 * j + 3]);
-        ml_sh[wave * 64 + lane] = make_float2(m, sum);
-    }
-    __syncthreads();
-    if (half == 0) {
-        const float2 e = ml_sh[wave * 64 + lane];
-        const float top = fmaxf(m, e.x);
-        const float f0 = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - top);
-        const float f1 = e.x == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(e.x - top);
-        m = top;
-        sum = sum * f0 + e.y * f1;
-#pragma unroll
-        for (int dt = 0; dt < kDt; dt++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const float4 w = o_sh[(dt * 4 + j) * 256];
-                o[dt][4 * j] = o[dt][4 * j] * f0 + w.x * f1;
-                o[dt][4 * j + 1] = o[dt][4 * j + 1] * f0 + w.y * f1;
-                o[dt][4 * j + 2] = o[dt][4 * j + 2] * f0 + w.z * f1;
-                o[dt][4 * j + 3] = o[dt][4 * j + 3] * f0 + w.w * f1;
-            }
-    }
-    if (half == 0 && first + c < t.n_rows && (only < 0 || only == my_tok)) {
+    if (first + c < t.n_rows && (only < 0 || only == my_tok)) {
 
     // lane (c, h): row c, values 32 dt + 8 j + 4 h + i
     const int tok = t.first_row + my_tok, qh = head * a.group + my % a.group;
@@ -973,8 +974,24 @@ __global__ __launch_bounds__(512, 2) void k_paged_rows(AttnArgs a)
     }
     if (only < 0 || only == t.tok_hi) return;
     only++;
-    __syncthreads();  // the sums are read before the buffers are written again
     }
+}
+
+// Both kinds of tiles in one launch, the longer ones first: what reads pages
+// for a few rows runs beside what computes.
+struct MixedArgs {
+    AttnArgs rows, few;
+    int row_blocks;
+};
+template <int D, int CDT, int QDT>
+__global__ __launch_bounds__(256, 2) void k_paged_mixed(MixedArgs a)
+{
+    __shared__ union {
+        SharedRows<D> rows;
+        Shared16<D> few;
+    } sh;
+    if ((int)blockIdx.x < a.row_blocks) attn_rows<D, CDT, QDT>(a.rows, blockIdx.x, sh.rows);
+    else attn16<D, CDT, QDT>(a.few, blockIdx.x - a.row_blocks, sh.few);
 }
 
 // ---- parts joined ----------------------------------------------------------------
@@ -982,9 +999,8 @@ __global__ __launch_bounds__(512, 2) void k_paged_rows(AttnArgs a)
 // A row's parts in their order, sixteen rows a workgroup: the rows of tiles of
 // M rows that visit their positions in steps of S.
 template <int D, int M, int S>
-__global__ __launch_bounds__(16 * D / 8) void k_paged_join(AttnArgs a)
+__device__ __forceinline__ void join_parts(const AttnArgs& a, int b)
 {
-    int b = blockIdx.x;
     const int head = b % a.hkv;
     b /= a.hkv;
     Tile t;
@@ -1028,6 +1044,18 @@ __global__ __launch_bounds__(16 * D / 8) void k_paged_join(AttnArgs a)
 #pragma unroll
     for (int i = 0; i < 8; i++) r[i] *= inv;
     store_out<D>(a, tok, qh, c8, r);
+}
+
+template <int D>
+__global__ __launch_bounds__(16 * D / 8) void k_paged_join(AttnArgs a)
+{
+    join_parts<D, 16, 32>(a, blockIdx.x);
+}
+template <int D>
+__global__ __launch_bounds__(16 * D / 8) void k_paged_join_mixed(MixedArgs a)
+{
+    if ((int)blockIdx.x < a.row_blocks) join_parts<D, kRowsM, rows_step(D)>(a.rows, blockIdx.x);
+    else join_parts<D, 16, 32>(a.few, blockIdx.x - a.row_blocks);
 }
 
 // ---- launches -----------------------------------------------------------------
@@ -1140,15 +1168,18 @@ static int attn_launch(const AttnPlan& p, hipStream_t st)
                  "paged_attn: %lld tiles of %d parts are too many for one launch", tiles > slots ? tiles : slots,
                  f.splits_max);
     if (p.some_rows) {
-        hipLaunchKernelGGL((k_paged_rows<D, CDT, QDT>), dim3((unsigned)(slots * r.splits)), dim3(512), 0, st, r);
-        if (r.splits > 1)
-            hipLaunchKernelGGL((k_paged_join<D, kRowsM, rows_step(D)>), dim3((unsigned)(slots * (kRowsM / 16))),
-                               dim3(16 * D / 8), 0, st, r);
+        MixedArgs m{r, f, (int)(slots * r.splits)};
+        hipLaunchKernelGGL((k_paged_mixed<D, CDT, QDT>), dim3((unsigned)(m.row_blocks + tiles * f.splits)), dim3(256), 0,
+                           st, m);
+        if (f.splits_max > 1) {
+            m.row_blocks = r.splits > 1 ? (int)(slots * (kRowsM / 16)) : 0;
+            const unsigned blocks = (unsigned)(m.row_blocks + (f.splits > 1 ? tiles : 0));
+            hipLaunchKernelGGL((k_paged_join_mixed<D>), dim3(blocks), dim3(16 * D / 8), 0, st, m);
+        }
+        return launch_status("k_paged_mixed");
     }
-    const dim3 grid((unsigned)(tiles * f.splits));
-    hipLaunchKernelGGL((k_paged_attn16<D, CDT, QDT>), grid, dim3(256), 0, st, f);
-    if (f.splits > 1)
-        hipLaunchKernelGGL((k_paged_join<D, 16, 32>), dim3((unsigned)tiles), dim3(16 * D / 8), 0, st, f);
+    hipLaunchKernelGGL((k_paged_attn16<D, CDT, QDT>), dim3((unsigned)(tiles * f.splits)), dim3(256), 0, st, f);
+    if (f.splits > 1) hipLaunchKernelGGL((k_paged_join<D>), dim3((unsigned)tiles), dim3(16 * D / 8), 0, st, f);
     return launch_status("k_paged_attn16");
 }
 
