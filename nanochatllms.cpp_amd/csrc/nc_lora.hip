@@ -1,10 +1,22 @@
 // nc_lora.hip -- low-rank adapters of many requests beside a shared
 // projection: out = base + scale (x a^T) b^T, each request with its own.
+//
+// The kernel computes t^T = a x^T and then out^T = b t^T on the matrix cores,
+// sixteen rows of one request at a time: in the output layout a lane
+// then holds ranks 16 i + 4 g + j (g = lane / 16, j < 4) of row lane % 16,
+// and with the ranks of the second product taken in that order (its factor b
+// is read so) those are already its operand.
+//
+// t has to enter the second product in fp16: it is split into a high and a
+// low half (t = hi + lo to 2^-22 of the row's largest, after scaling the row
+// by a power of two), so the product is as good as an fp32 one.  x's Q8 codes
+// are exact in fp16, and a block's sum is multiplied by its delta in fp32.
 #include "nc_act.h"
 #include "nc_paged.h"
 
 namespace nc {
 
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
@@ -17,208 +29,362 @@ struct LoraArgs {
     uint8_t* out;
     int x_pitch, base_pitch, out_pitch;
     int n_adapters, rank, k, n, n_req, max_tokens, max_new;
-    int chunk;  // columns of a workgroup, a multiple of 128
+    int chunk;  // columns of a workgroup, a multiple of 64
 };
 
-// Eight ranks of a row of a or b from `at` on, zero past `rank`.
-__device__ __forceinline__ half8 rank8(const uint16_t* row, int at, int rank)
+// A matrix operand wants one row from each of sixteen lanes side by side; so
+// loaded, every lane is an access of its own to the first-level cache (62 per
+// load instruction were counted, and bound the kernel).  Operands therefore
+// come as whole stretches of rows and go through a wavefront's own piece of
+// shared memory, sixteen bytes at a time, pieces exchanged within rows by the
+// row's number so that neither side meets in a bank.  No barrier: a
+// wavefront's accesses to it keep their order.
+__device__ __forceinline__ int place16(int row, int piece) { return (row * 16 + (piece ^ row)) * 16; }  // of 256 B rows
+__device__ __forceinline__ int place8(int row, int piece) { return (row * 8 + (piece ^ (row >> 1 & 7))) * 16; }  // of 128 B
+
+// Piece of a row of RT * 32 bytes.
+template <int RT>
+__device__ __forceinline__ int place_b(int row, int piece)
 {
-    if ((rank & 7) == 0) {
-        half8 z = {};
-        return at < rank ? *reinterpret_cast<const half8*>(row + at) : z;
-    }
-    half8 v;
-#pragma unroll
-    for (int i = 0; i < 8; i++)
-        v[i] = at + i < rank ? __builtin_bit_cast(_Float16, row[min(at + i, rank - 1)]) : (_Float16)0.0f;
-    return v;
+    return (row * (2 * RT) + (piece ^ (row / (8 / RT) & (2 * RT - 1)))) * 16;
 }
 
-// One workgroup: sixteen rows of one request times `chunk` columns.  First
-// the rows' low-rank products t = a x, as t^T = a x^T on the matrix cores
-// with the four wavefronts taking every fourth 32 of k, summed in shared
-// memory; then 32 columns at a time per wavefront, out^T = b t^T, the base
-// added and the result stored by the lane that holds it.
-//
-// t has to enter the second product in fp16: it is split into a high and a
-// low half (t = hi + lo to 2^-22 of the row's largest, after scaling the row
-// by a power of two), so the product is as good as fp32 ones.  x's Q8 codes
-// are exact in fp16 and a block's sum is multiplied by its delta in fp32.
-template <int XDT, int ODT, int RT>
-__global__ __launch_bounds__(256) void k_lora(LoraArgs a)
+// 128 of k (from k0) of sixteen rows of a: lane l loads sixteen bytes of rows
+// l / 16 + 4 i; rows past the rank repeat the last, and b has nothing for them.
+__device__ __forceinline__ void load_a(const LoraArgs& a, const uint16_t* wa, int rank0, int k0, int lane, uint4 (&v)[4])
 {
-    constexpr int kR = RT * 16, kKs = (RT + 1) / 2, kTp = kKs * 32 + 4;
-    __shared__ float part[4][16][kTp];
+    const int k = k0 + lane % 16 * 8;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t r = min(rank0 + lane / 16 + 4 * i, a.rank - 1);
+        v[i] = k < a.k ? *reinterpret_cast<const uint4*>(wa + (size_t)(r * (uint32_t)a.k) + k) : make_uint4(0, 0, 0, 0);
+    }
+}
+__device__ __forceinline__ void put16(uint8_t* sh, int lane, const uint4 (&v)[4])
+{
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int row = lane / 16 + 4 * i;
+        *reinterpret_cast<uint4*>(sh + place16(row, lane % 16)) = v[i];
+    }
+}
+
+// The workgroup's sixteen rows; rows past the request's end repeat its last.
+struct LoraRows {
+    int id;     // the adapter, -1 for none
+    int first;  // row of the tensors
+    int n;      // rows, 1 to 16
+    __device__ __forceinline__ int at(int i) const { return first + min(i, n - 1); }
+};
+
+// The same 128 of k of the sixteen rows of x (and, of Q8 rows, lane l's row
+// l % 16's four deltas).
+template <int XDT>
+struct XPiece {
+    uint4 v[XDT == F16 ? 4 : 2];
+    uint2 d;
+    __device__ __forceinline__ void load(const LoraArgs& a, const LoraRows& w, int k0, int lane)
+    {
+        constexpr int kPer = XDT == F16 ? 16 : 8, kE = XDT == F16 ? 8 : 16;  // lanes of a row, values of a lane
+        const int k = k0 + lane % kPer * kE;
+#pragma unroll
+        for (int i = 0; i < (XDT == F16 ? 4 : 2); i++) {
+            const uint8_t* row = a.x + (size_t)w.at(lane / kPer + i * (64 / kPer)) * a.x_pitch;
+            v[i] = make_uint4(0, 0, 0, 0);
+            if (k < a.k) v[i] = *reinterpret_cast<const uint4*>(row + k * (XDT == F16 ? 2 : 1));
+        }
+        if constexpr (XDT == Q8) {
+            const uint8_t* row = a.x + (size_t)w.at(lane % 16) * a.x_pitch + a.k;
+            d = make_uint2(0, 0);
+            if (k0 + 128 <= a.k) {
+                d = *reinterpret_cast<const uint2*>(row + k0 / 16);
+            } else {
+                const uint16_t* p = reinterpret_cast<const uint16_t*>(row + k0 / 16);
+                const int n = (a.k - k0) / 32;  // 1 to 3, or none
+                if (n > 0) d.x = p[0];
+                if (n > 1) d.x |= (uint32_t)p[1] << 16;
+                if (n > 2) d.y = p[2];
+            }
+        }
+    }
+    // Operands of the four 32s.
+    __device__ __forceinline__ void operands(uint8_t* sh, int lane, half8 (&x)[4]) const
+    {
+        const int c = lane & 15, g = lane >> 4;
+        if constexpr (XDT == F16) {
+            put16(sh, lane, v);
+#pragma unroll
+            for (int ks = 0; ks < 4; ks++) x[ks] = *reinterpret_cast<const half8*>(sh + place16(c, ks * 4 + g));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+                *reinterpret_cast<uint4*>(sh + place8(lane / 8 + 8 * i, lane % 8)) = v[i];
+#pragma unroll
+            for (int ks = 0; ks < 4; ks++) {
+                const uint2 q = *reinterpret_cast<const uint2*>(sh + place8(c, ks * 2 + (g >> 1)) + (g & 1) * 8);
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    x[ks][i] = (_Float16)(float)(int8_t)((i < 4 ? q.x >> (8 * i) : q.y >> (8 * (i - 4))) & 0xFFu);
+            }
+        }
+    }
+    __device__ __forceinline__ float delta(int ks) const
+    {
+        const uint32_t p = ks < 2 ? d.x : d.y;
+        return h2f((uint16_t)(ks & 1 ? p >> 16 : p & 0xFFFFu));
+    }
+};
+
+// t as the operands of the second product, and what to multiply it by.
+template <int RT>
+__device__ __forceinline__ float split_low_rank(const f32x4 (&t)[RT], float scale, half8 (&hi)[(RT + 1) / 2],
+                                                half8 (&lo)[(RT + 1) / 2])
+{
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < RT; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) top = fmaxf(top, fabsf(t[i][j]));
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    // the row's largest to [2^13, 2^14)
+    const int e = top > 0.0f && top < __builtin_inff() ? 13 - ilogbf(top) : 0;
+#pragma unroll
+    for (int i = 0; i < 2 * ((RT + 1) / 2); i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float f = i < RT ? ldexpf(t[i < RT ? i : 0][j], e) : 0.0f;
+            const _Float16 h = (_Float16)f;
+            hi[i / 2][4 * (i & 1) + j] = h;
+            lo[i / 2][4 * (i & 1) + j] = (_Float16)(fabsf(f) < __builtin_inff() ? f - (float)h : 0.0f);
+        }
+    return ldexpf(scale, -e);
+}
+
+// Columns [n, n + 32) of b as eight-byte pieces of four ranks in shared
+// memory, zero past the rank: rows of RT * 32 bytes, which are the same bytes
+// in memory where the rank is RT * 16.
+template <int RT>
+__device__ __forceinline__ void put_b(const LoraArgs& a, const uint16_t* wb, int n, int lane, uint8_t* sh)
+{
+    constexpr int kRow = RT * 32;  // bytes
+    if (a.rank == RT * 16) {
+        constexpr int kN = RT;  // 32 rows of them in 1 KB loads
+        const uint8_t* src = reinterpret_cast<const uint8_t*>(wb + (size_t)n * a.rank);
+        const int left = min(a.n - n, 32) * kRow;  // bytes of b from here on
+        uint4 v[kN];
+#pragma unroll
+        for (int i = 0; i < kN; i++) {
+            const int at = (i * 64 + lane) * 16;
+            v[i] = at < left ? *reinterpret_cast<const uint4*>(src + at) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < kN; i++) {
+            const int at = i * 64 + lane;
+            *reinterpret_cast<uint4*>(sh + place_b<RT>(at / (2 * RT), at % (2 * RT))) = v[i];
+        }
+        return;
+    }
+    // another rank: one row from each pair of lanes
+    const int col = lane / 2;
+    const uint16_t* row = wb + (size_t)min(n + col, a.n - 1) * a.rank;
+    for (int at = lane % 2 * 4; at < RT * 16; at += 8) {
+        uint32_t p[2] = {0, 0};
+        if ((a.rank & 3) == 0) {
+            if (at < a.rank) {
+                const uint2 w = *reinterpret_cast<const uint2*>(row + at);
+                p[0] = w.x, p[1] = w.y;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (at + j < a.rank) p[j >> 1] |= (uint32_t)row[at + j] << (16 * (j & 1));
+        }
+        *reinterpret_cast<uint2*>(sh + place_b<RT>(col, at / 8) + at % 8 * 2) = make_uint2(p[0], p[1]);
+    }
+}
+
+// Four columns from `col` on of one row: base plus y, stored.  Of Q8 rows
+// eight lanes side by side hold a block.
+template <int ODT>
+__device__ __forceinline__ void store4(const LoraArgs& a, uint8_t* op, int col, int n1, bool live, float4 r)
+{
+    const float v[4] = {r.x, r.y, r.z, r.w};
+    if constexpr (ODT == Q8) {
+        float top = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (col + j < n1) top = fmaxf(top, fabsf(v[j]));
+        top = quad_max(top);
+        top = fmaxf(top, dpp_f<0x141>(top));  // row_half_mirror: the other quad of the eight
+        const float delta = top / 127.0f, inv = delta != 0.0f ? 1.0f / delta : 0.0f;
+        if (!live || (col & ~31) >= n1) return;
+        uint32_t w = 0;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int8_t q = col + j < n1 ? (int8_t)roundf(v[j] * inv) : (int8_t)0;
+            w |= (uint32_t)(uint8_t)q << (8 * j);
+        }
+        *reinterpret_cast<uint32_t*>(op + col) = w;  // codes come in whole blocks
+        if ((col & 31) == 0) reinterpret_cast<uint16_t*>(op + act_delta_offset(a.n))[col >> 5] = f2h(delta);
+    } else {
+        if (!live || col >= n1) return;
+        if constexpr (ODT == F32) {
+            float* o = reinterpret_cast<float*>(op) + col;
+            if (col + 4 <= n1) {
+                *reinterpret_cast<float4*>(o) = r;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 3; j++)
+                    if (col + j < n1) o[j] = v[j];
+            }
+        } else {
+            uint16_t* o = reinterpret_cast<uint16_t*>(op) + col;
+            if (col + 4 <= n1) {
+                *reinterpret_cast<uint2*>(o) = make_uint2((uint32_t)f2h(v[0]) | (uint32_t)f2h(v[1]) << 16,
+                                                          (uint32_t)f2h(v[2]) | (uint32_t)f2h(v[3]) << 16);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 3; j++)
+                    if (col + j < n1) o[j] = f2h(v[j]);
+            }
+        }
+    }
+}
+
+constexpr int lora_waves(int rt) { return rt >= 4 ? 8 : 16; }
+constexpr int lora_piece(int rt) { return rt == 8 ? 8192 : 4096; }  // bytes of shared memory of a wavefront
+
+// One workgroup for sixteen rows and `chunk` columns.  Its wavefronts share
+// out k by 128s, and sum t in shared memory; then each takes 64 columns at a
+// time.  t is made again for every chunk, so chunks are few and workgroups
+// large.
+template <int XDT, int ODT, int RT>
+__global__ __launch_bounds__(64 * lora_waves(RT)) void k_lora(LoraArgs a)
+{
+    constexpr int kW = lora_waves(RT), kT = RT * 256, kKs = (RT + 1) / 2;
+    __shared__ __align__(16) uint8_t piece[kW][lora_piece(RT)];
+    __shared__ __align__(16) float whole[kT];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 15, g = lane >> 4;
+    uint8_t* const sh = piece[wave];
     const int tile = blockIdx.x;
-    const int req = tile_request(a.row_start, a.n_req, tile, 1, 16, a.max_tokens);
-    const RowSpan s = request_rows(a.row_start, req, a.max_tokens, a.max_new);
-    const int row0 = (tile - first_tile(a.row_start[req], req, 1, 16, a.max_tokens)) * 16;
+    const TileRequest at = tile_request(a.row_start, a.adapter, a.n_req, tile, 1, 16, a.max_tokens);
+    RowSpan s = request_rows(at.start, at.end, a.max_tokens);
+    s.n = min(s.n, a.max_new);
+    const int row0 = (tile - first_tile(at.start, at.req, 1, 16, a.max_tokens)) * 16;
     if (row0 < 0 || row0 >= s.n) return;
-    const int id = a.adapter[req];
-    const bool some = (unsigned)id < (unsigned)a.n_adapters;
-    const bool live = row0 + c < s.n;
-    const int row = s.first + min(row0 + c, s.n - 1);
+    const LoraRows w{(unsigned)at.of < (unsigned)a.n_adapters ? at.of : -1, s.first + row0, min(s.n - row0, 16)};
+    const int n0 = blockIdx.y * a.chunk + wave * 64, n1 = min((int)(blockIdx.y + 1) * a.chunk, a.n);
 
+    // lane l: four columns from 4 (l % 16) on of rows l / 16 + 4 i
+    auto load_base = [&](float4 (&v)[4], int n) {
+        const int col = n + lane % 16 * 4;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float* p = reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(a.base) +
+                                                            (size_t)w.at(lane / 16 + 4 * i) * a.base_pitch) + col;
+            v[i] = make_float4(0, 0, 0, 0);
+            if (col + 4 <= n1) {
+                v[i] = *reinterpret_cast<const float4*>(p);  // col is a multiple of 4
+            } else {
+                if (col < n1) v[i].x = p[0];
+                if (col + 1 < n1) v[i].y = p[1];
+                if (col + 2 < n1) v[i].z = p[2];
+            }
+        }
+    };
+    float4 base[4];
+    if (n0 < n1) load_base(base, n0);
     float unit = 0.0f;
     half8 hi[kKs], lo[kKs];
-    if (some) {
-        const uint16_t* wa = a.a + (size_t)id * a.rank * a.k;
-        const uint8_t* x = a.x + (size_t)row * a.x_pitch;
+    if (w.id >= 0) {
+        const uint16_t* wa = a.a + (size_t)w.id * a.rank * a.k;
+        const float scale = a.scale[w.id];
         f32x4 t[RT];
 #pragma unroll
         for (int i = 0; i < RT; i++) t[i] = f32x4{0, 0, 0, 0};
-        const int steps = a.k / 32;
-#pragma unroll 4
-        for (int ks = wave; ks < steps; ks += 4) {
-            half8 xv;
-            float d = 1.0f;
-            if constexpr (XDT == Q8) {
-                const uint2 q = *reinterpret_cast<const uint2*>(x + ks * 32 + g * 8);
-                d = h2f(reinterpret_cast<const uint16_t*>(x + a.k)[ks]);
+        for (int k0 = wave * 128; k0 < a.k; k0 += kW * 128) {
+            constexpr int kAhead = RT < 2 ? RT : 2;  // sixteens of ranks on their way
+            XPiece<XDT> xp;
+            uint4 av[kAhead][4];
+            xp.load(a, w, k0, lane);
 #pragma unroll
-                for (int i = 0; i < 8; i++)
-                    xv[i] = (_Float16)(float)(int8_t)((i < 4 ? q.x >> (8 * i) : q.y >> (8 * (i - 4))) & 0xFFu);
-            } else {
-                xv = *reinterpret_cast<const half8*>(x + (ks * 32 + g * 8) * 2);
-            }
+            for (int i = 0; i < kAhead; i++) load_a(a, wa, i * 16, k0, lane, av[i]);
+            half8 x[4];
+            xp.operands(sh, lane, x);
 #pragma unroll
             for (int i = 0; i < RT; i++) {
-                const int r = i * 16 + c;
-                half8 av = {};
-                if (r < a.rank) av = *reinterpret_cast<const half8*>(wa + (size_t)r * a.k + ks * 32 + g * 8);
-                if constexpr (XDT == Q8) {
-                    const f32x4 z = {0, 0, 0, 0};
-                    const f32x4 p = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, xv, z, 0, 0, 0);
+                put16(sh, lane, av[i % kAhead]);
+                if (i + kAhead < RT) load_a(a, wa, (i + kAhead) * 16, k0, lane, av[i % kAhead]);
 #pragma unroll
-                    for (int j = 0; j < 4; j++) t[i][j] = __builtin_fmaf(p[j], d, t[i][j]);
-                } else {
-                    t[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, xv, t[i], 0, 0, 0);
+                for (int ks = 0; ks < 4; ks++) {
+                    const half8 f = *reinterpret_cast<const half8*>(sh + place16(c, ks * 4 + g));
+                    if constexpr (XDT == Q8) {
+                        const f32x4 p = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, x[ks], f32x4{0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+                        for (int j = 0; j < 4; j++) t[i][j] = __builtin_fmaf(p[j], xp.delta(ks), t[i][j]);
+                    } else {
+                        t[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, x[ks], t[i], 0, 0, 0);
+                    }
                 }
             }
         }
-        // lane (c, g): row c, ranks 16 i + 4 g + j
 #pragma unroll
-        for (int i = 0; i < RT; i++)
-            *reinterpret_cast<f32x4*>(&part[wave][c][i * 16 + 4 * g]) = t[i];
-        if constexpr (RT & 1)
-            *reinterpret_cast<f32x4*>(&part[wave][c][kR + 4 * g]) = f32x4{0, 0, 0, 0};
+        for (int i = 0; i < RT; i++) *reinterpret_cast<f32x4*>(sh + (i * 64 + lane) * 16) = t[i];
         __syncthreads();
-        float v[kKs][8], top = 0.0f;
+        for (int e = tid; e < kT; e += 64 * kW) {
+            float sum = 0.0f;
 #pragma unroll
-        for (int ks = 0; ks < kKs; ks++)
+            for (int i = 0; i < kW; i++) sum += reinterpret_cast<const float*>(piece[i])[e];
+            whole[e] = sum;
+        }
+        __syncthreads();
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const int r = ks * 32 + g * 8 + j;
-                v[ks][j] = (part[0][c][r] + part[1][c][r]) + (part[2][c][r] + part[3][c][r]);
-                top = fmaxf(top, fabsf(v[ks][j]));
-            }
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        // the row's largest to [2^13, 2^14)
-        const int e = top > 0.0f && top < __builtin_inff() ? 14 - (ilogbf(top) + 1) : 0;
-        unit = ldexpf(a.scale[id], -e);
-#pragma unroll
-        for (int ks = 0; ks < kKs; ks++)
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const float f = ldexpf(v[ks][j], e);
-                hi[ks][j] = (_Float16)f;
-                const float rest = f - (float)hi[ks][j];
-                lo[ks][j] = (_Float16)(fabsf(f) < __builtin_inff() ? rest : 0.0f);
-            }
+        for (int i = 0; i < RT; i++) t[i] = *reinterpret_cast<const f32x4*>(&whole[(i * 64 + lane) * 4]);
+        unit = split_low_rank<RT>(t, scale, hi, lo);
     }
-    const uint16_t* wb = a.b + (some ? (size_t)id * a.n * a.rank : 0);
-    const int n0 = blockIdx.y * a.chunk, n1 = min(n0 + a.chunk, a.n);
-    const bool vec = (a.n & 3) == 0;
-    for (int n = n0 + wave * 32; n < n1; n += 128) {
-        f32x4 y[2];
+    const uint16_t* wb = a.b + (w.id >= 0 ? (size_t)w.id * a.n * a.rank : 0);
+    for (int n = n0; n < n1; n += 64 * kW) {
+        float4 r[4];
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
-            y[u] = f32x4{0, 0, 0, 0};
-            if (some) {
-                const int col = min(n + u * 16 + c, a.n - 1);
+        for (int i = 0; i < 4; i++) r[i] = base[i];
+        if (n + 64 * kW < n1) load_base(base, n + 64 * kW);
+        if (w.id >= 0) {
+            f32x4 y[4];
 #pragma unroll
-                for (int ks = 0; ks < kKs; ks++) {
-                    const half8 bv = rank8(wb + (size_t)col * a.rank, ks * 32 + g * 8, a.rank);
-                    y[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bv, hi[ks], y[u], 0, 0, 0);
-                    y[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bv, lo[ks], y[u], 0, 0, 0);
-                }
-            }
-        }
-        // lane (c, g): row c, columns n + 16 u + 4 g + j
-        const float* bp = reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(a.base) +
-                                                         (size_t)row * a.base_pitch);
-        uint8_t* op = a.out + (size_t)row * a.out_pitch;
-        float r[2][4];
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-            const int col = n + u * 16 + 4 * g;
-            float bv[4] = {};
-            if (vec && col < n1) {
-                const float4 w = *reinterpret_cast<const float4*>(bp + col);
-                bv[0] = w.x, bv[1] = w.y, bv[2] = w.z, bv[3] = w.w;
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    if (col + j < n1) bv[j] = bp[col + j];
-            }
-#pragma unroll
-            for (int j = 0; j < 4; j++) r[u][j] = some ? __builtin_fmaf(y[u][j], unit, bv[j]) : bv[j];
-        }
-        if constexpr (ODT == Q8) {
-            // the 32 columns are one block, on the lanes of the row
-            float top = 0.0f;
-#pragma unroll
-            for (int u = 0; u < 2; u++)
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    if (n + u * 16 + 4 * g + j < n1) top = fmaxf(top, fabsf(r[u][j]));
-            top = fmaxf(top, __shfl_xor(top, 16));
-            top = fmaxf(top, __shfl_xor(top, 32));
-            const float delta = top / 127.0f;
-            const float inv = delta != 0.0f ? 1.0f / delta : 0.0f;
-            if (live) {
+            for (int h = 0; h < 2; h++) {
+                if (n + 32 * h < n1) put_b<RT>(a, wb, n + 32 * h, lane, sh);
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
-                    const int col = n + u * 16 + 4 * g;
-                    uint32_t w = 0;
+                    y[2 * h + u] = f32x4{0, 0, 0, 0};
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const int8_t q = col + j < n1 ? (int8_t)roundf(r[u][j] * inv) : (int8_t)0;
-                        w |= (uint32_t)(uint8_t)q << (8 * j);
-                    }
-                    *reinterpret_cast<uint32_t*>(op + col) = w;  // codes come in whole blocks
-                }
-                if (g == 0) reinterpret_cast<uint16_t*>(op + act_delta_offset(a.n))[n >> 5] = f2h(delta);
-            }
-        } else if (live) {
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const int col = n + u * 16 + 4 * g;
-                if (ODT == F32) {
-                    float* o = reinterpret_cast<float*>(op) + col;
-                    if (vec && col < n1) {
-                        *reinterpret_cast<float4*>(o) = make_float4(r[u][0], r[u][1], r[u][2], r[u][3]);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 4; j++)
-                            if (col + j < n1) o[j] = r[u][j];
-                    }
-                } else {
-                    uint16_t* o = reinterpret_cast<uint16_t*>(op) + col;
-                    if (vec && col < n1) {
-                        *reinterpret_cast<uint2*>(o) =
-                            make_uint2((uint32_t)f2h(r[u][0]) | (uint32_t)f2h(r[u][1]) << 16,
-                                       (uint32_t)f2h(r[u][2]) | (uint32_t)f2h(r[u][3]) << 16);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 4; j++)
-                            if (col + j < n1) o[j] = f2h(r[u][j]);
+                    for (int ks = 0; ks < kKs; ks++) {
+                        // ranks 32 ks + 4 g + j, and 16 more
+                        auto four = [&](int piece) {
+                            return *reinterpret_cast<const uint2*>(sh + place_b<RT>(u * 16 + c, piece) + (g & 1) * 8);
+                        };
+                        const uint2 q0 = four(4 * ks + (g >> 1));
+                        const uint2 q1 = 2 * ks + 1 < RT ? four(4 * ks + 2 + (g >> 1)) : make_uint2(0, 0);
+                        const half8 f = __builtin_bit_cast(half8, u32x4{q0.x, q0.y, q1.x, q1.y});
+                        y[2 * h + u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, hi[ks], y[2 * h + u], 0, 0, 0);
+                        y[2 * h + u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, lo[ks], y[2 * h + u], 0, 0, 0);
                     }
                 }
             }
+            // from row l % 16, columns 16 u + 4 (l / 16) on, to the base's lanes
+#pragma unroll
+            for (int u = 0; u < 4; u++) *reinterpret_cast<f32x4*>(sh + place16(c, u * 4 + g)) = y[u] * unit;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float4 v = *reinterpret_cast<const float4*>(sh + place16(lane / 16 + 4 * i, lane % 16));
+                r[i] = make_float4(r[i].x + v.x, r[i].y + v.y, r[i].z + v.z, r[i].w + v.w);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int row = lane / 16 + 4 * i;
+            store4<ODT>(a, a.out + (size_t)w.at(row) * a.out_pitch, n + lane % 16 * 4, n1, row < w.n, r[i]);
         }
     }
 }
@@ -226,10 +392,10 @@ __global__ __launch_bounds__(256) void k_lora(LoraArgs a)
 template <int XDT, int ODT>
 static void lora_launch(const LoraArgs& a, dim3 grid, hipStream_t st)
 {
-    if (a.rank <= 16) hipLaunchKernelGGL((k_lora<XDT, ODT, 1>), grid, dim3(256), 0, st, a);
-    else if (a.rank <= 32) hipLaunchKernelGGL((k_lora<XDT, ODT, 2>), grid, dim3(256), 0, st, a);
-    else if (a.rank <= 64) hipLaunchKernelGGL((k_lora<XDT, ODT, 4>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((k_lora<XDT, ODT, 8>), grid, dim3(256), 0, st, a);
+    if (a.rank <= 16) hipLaunchKernelGGL((k_lora<XDT, ODT, 1>), grid, dim3(64 * lora_waves(1)), 0, st, a);
+    else if (a.rank <= 32) hipLaunchKernelGGL((k_lora<XDT, ODT, 2>), grid, dim3(64 * lora_waves(2)), 0, st, a);
+    else if (a.rank <= 64) hipLaunchKernelGGL((k_lora<XDT, ODT, 4>), grid, dim3(64 * lora_waves(4)), 0, st, a);
+    else hipLaunchKernelGGL((k_lora<XDT, ODT, 8>), grid, dim3(64 * lora_waves(8)), 0, st, a);
 }
 
 }  // namespace nc
@@ -242,7 +408,7 @@ extern "C" int nc_lora_add(const nc_tensor* x, const nc_tensor* base, const nc_l
     NC_CHECK_ARG(lora && lora->a && lora->b && lora->scale && adapter && row_start, "lora_add: null argument");
     NC_CHECK_ARG(lora->rank >= 1 && lora->rank <= NC_LORA_MAX_RANK, "lora_add: rank %d (1 to %d)", lora->rank,
                  NC_LORA_MAX_RANK);
-    NC_CHECK_ARG(lora->k >= 32 && lora->k % 32 == 0 && lora->n >= 1 && lora->n_adapters >= 1,
+    NC_CHECK_ARG(lora->k >= 32 && lora->k % 32 == 0 && lora->k <= (1 << 24) && lora->n >= 1 && lora->n_adapters >= 1,
                  "lora_add: %d adapters [%d, %d] (k a multiple of 32)", lora->n_adapters, lora->n, lora->k);
     NC_CHECK_ARG(aligned16(lora->a) && aligned16(lora->b), "lora_add: adapters are not 16-byte aligned");
     NC_CHECK_ARG(n_req >= 1 && n_req <= NC_PAGED_MAX_REQ && max_new >= 0, "lora_add: %d requests of %d rows", n_req,
@@ -275,12 +441,15 @@ extern "C" int nc_lora_add(const nc_tensor* x, const nc_tensor* base, const nc_l
     a.max_tokens = rows;
     a.max_new = max_new;
     const long long tiles = tile_slots(rows, n_req, 1, 16);
-    long long chunks = (1024 + tiles - 1) / tiles;
-    const long long cap = ((long long)a.n + 127) / 128;
+    const long long work = max_new == 1 ? n_req : rows / 16 + 1;  // tiles that hold rows, about
+    long long chunks = 512 / work;
+    const int most = 64 * lora_waves(a.rank > 32 ? 8 : 1);
+    const long long cap = ((long long)a.n + most - 1) / most;  // few wavefronts without columns
     if (chunks > cap) chunks = cap;
     if (chunks < 1) chunks = 1;
-    a.chunk = (int)(((a.n + chunks - 1) / chunks + 127) / 128 * 128);
+    a.chunk = (int)(((a.n + chunks - 1) / chunks + 63) / 64 * 64);
     const dim3 grid((unsigned)tiles, (unsigned)((a.n + a.chunk - 1) / a.chunk));
+    NC_CHECK_ARG(grid.y <= 65535 && tiles <= 0xFFFFFF, "lora_add: %d columns are too many", a.n);
     hipStream_t st = stream_of(stream);
     if (x->dtype == NC_Q8) {
         if (out->dtype == NC_Q8) lora_launch<Q8, Q8>(a, grid, st);

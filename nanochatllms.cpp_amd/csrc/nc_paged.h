@@ -19,16 +19,15 @@ inline bool paged_rows_ok(const nc_tensor* t, int rows, int cols)
 int check_cache(const char* what, const nc_paged_cache* c);
 int check_batch(const char* what, const nc_paged_batch* b, int page_size);
 
-// Rows [first, first + n) of request r, clamped to the step's rows so that no
+// Rows [first, first + n) of a request, clamped to the step's rows so that no
 // table, however wrong, leads outside the tensors.
 struct RowSpan {
     int first, n;
 };
-__device__ __forceinline__ RowSpan request_rows(const int* row_start, int r, int max_tokens, int max_new)
+__device__ __forceinline__ RowSpan request_rows(int start, int end, int max_tokens)
 {
-    const int a = min(max(row_start[r], 0), max_tokens);
-    const int b = min(max(row_start[r + 1], 0), max_tokens);
-    return {a, min(max(b - a, 0), max_new)};
+    const int a = min(max(start, 0), max_tokens), b = min(max(end, 0), max_tokens);
+    return {a, max(b - a, 0)};
 }
 
 // Work is cut into tiles of `m` units, a request's row holding `per_row`
@@ -47,21 +46,28 @@ inline long long tile_slots(int max_tokens, int n_req, int per_row, int m)
     return (long long)max_tokens * per_row / m + n_req;
 }
 
-// The request of tile number t: the last one whose first tile is at most t,
-// found by a wavefront that probes 64 requests at a time.
-__device__ __forceinline__ int tile_request(const int* row_start, int n_req, int t, int per_row, int m, int max_tokens)
+// The request of tile number t, the last one whose first tile is at most t,
+// found by a wavefront that probes 64 requests at a time; with it, read in
+// the same go, its row_start, the next one's, and of[request].
+struct TileRequest {
+    int req, start, end, of;
+};
+__device__ __forceinline__ TileRequest tile_request(const int* row_start, const int* of, int n_req, int t, int per_row,
+                                                    int m, int max_tokens)
 {
     const int lane = threadIdx.x & (kWave - 1);
     int lo = 0, len = n_req;
     while (true) {
         const int step = (len + kWave - 1) / kWave;
-        const int r = lo + lane * step;
-        const bool at = lane * step < len && first_tile(row_start[min(r, n_req - 1)], r, per_row, m, max_tokens) <= t;
-        const int c = __popcll(__ballot(at));
-        if (c == 0) return __builtin_amdgcn_readfirstlane(lo);  // tables that are no row starts
-        lo += (c - 1) * step;
+        const int r = min(lo + lane * step, n_req - 1);
+        const int start = row_start[r], end = row_start[r + 1], value = of[r];
+        const bool at = lane * step < len && first_tile(start, r, per_row, m, max_tokens) <= t;
+        const int c = max(__popcll(__ballot(at)), 1);  // tables that are no row starts: the first
+        if (step == 1)
+            return {__builtin_amdgcn_readfirstlane(lo + c - 1), __builtin_amdgcn_readlane(start, c - 1),
+                    __builtin_amdgcn_readlane(end, c - 1), __builtin_amdgcn_readlane(value, c - 1)};
+        lo = __builtin_amdgcn_readfirstlane(lo + (c - 1) * step);
         len = min(step, n_req - lo);
-        if (step == 1) return __builtin_amdgcn_readfirstlane(lo);
     }
 }
 

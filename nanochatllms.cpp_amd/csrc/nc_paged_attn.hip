@@ -88,10 +88,9 @@ struct Tile {
 };
 
 template <int M>
-__device__ __forceinline__ bool tile_of(const AttnArgs& a, int req, int row0, Tile& t)
+__device__ __forceinline__ bool tile_of(const AttnArgs& a, int start, int end, int kv, int row0, Tile& t)
 {
-    const RowSpan s = request_rows(a.row_start, req, a.max_tokens, 0x7FFFFFFF);
-    const int kv = a.kv_len[req];
+    const RowSpan s = request_rows(start, end, a.max_tokens);
     const int limit = (int)min((long long)a.max_pages << a.lps, (long long)a.max_kv);
     if (kv > limit || kv < s.n) return false;  // lengths beyond the bounds: the rows are left as they were
     t.n_rows = min(s.n, a.max_new) * a.group;
@@ -347,7 +346,9 @@ __device__ __forceinline__ void attn16(const AttnArgs& a, int b, Shared16<D>& sh
     b /= a.hkv;
     const int req = b / a.row_tiles;
     Tile t;
-    if (!tile_of<16>(a, req, (b % a.row_tiles) * 16, t) || t.n_rows > a.few) return;
+    if (!tile_of<16>(a, a.row_start[req], a.row_start[req + 1], a.kv_len[req], (b % a.row_tiles) * 16, t) ||
+        t.n_rows > a.few)
+        return;
     const Steps<32> steps(t.lo, t.hi, a.sink);
     const int v0 = part * a.part;
     if (v0 >= steps.count) return;
@@ -730,10 +731,10 @@ __device__ __forceinline__ void attn_rows(const AttnArgs& a, int b, SharedRows<D
     b /= a.hkv;
     const int part = b % a.splits;
     const int slot = b / a.splits;
-    const int req = tile_request(a.row_start, a.n_req, slot, a.group, kRowsM, a.max_tokens);  // uniform
-    const int row0 = (slot - first_tile(a.row_start[req], req, a.group, kRowsM, a.max_tokens)) * kRowsM;
+    const TileRequest at = tile_request(a.row_start, a.kv_len, a.n_req, slot, a.group, kRowsM, a.max_tokens);
+    const int req = at.req, row0 = (slot - first_tile(at.start, req, a.group, kRowsM, a.max_tokens)) * kRowsM;
     Tile t;
-    if (row0 < 0 || !tile_of<kRowsM>(a, req, row0, t) || t.n_rows <= a.few) return;
+    if (row0 < 0 || !tile_of<kRowsM>(a, at.start, at.end, at.of, row0, t) || t.n_rows <= a.few) return;
     const Steps<kS> steps(t.lo, t.hi, a.sink);
     const int v0 = part * a.part;
     if (v0 >= steps.count) return;
@@ -1004,32 +1005,36 @@ __device__ __forceinline__ void join_parts(const AttnArgs& a, int b)
     const int head = b % a.hkv;
     b /= a.hkv;
     Tile t;
-    int sub = 0, req, row0;
+    int sub = 0, row0;
+    TileRequest at;
     if (M == 16) {
-        req = b / a.row_tiles;
+        const int req = b / a.row_tiles;
+        at = {req, a.row_start[req], a.row_start[req + 1], a.kv_len[req]};
         row0 = (b % a.row_tiles) * 16;
     } else {
         sub = b % (M / 16);
         b /= M / 16;
-        req = tile_request(a.row_start, a.n_req, b, a.group, M, a.max_tokens);
-        row0 = (b - first_tile(a.row_start[req], req, a.group, M, a.max_tokens)) * M;
+        at = tile_request(a.row_start, a.kv_len, a.n_req, b, a.group, M, a.max_tokens);
+        row0 = (b - first_tile(at.start, at.req, a.group, M, a.max_tokens)) * M;
     }
-    if (row0 < 0 || !tile_of<M>(a, req, row0, t) || (M == 16 ? t.n_rows > a.few : t.n_rows <= a.few)) return;
+    if (row0 < 0 || !tile_of<M>(a, at.start, at.end, at.of, row0, t) ||
+        (M == 16 ? t.n_rows > a.few : t.n_rows <= a.few))
+        return;
     const Steps<S> steps(t.lo, t.hi, a.sink);
     const int parts = min((steps.count + a.part - 1) / a.part, a.splits);
     const int rr = threadIdx.x / (D / 8), c8 = threadIdx.x % (D / 8);
     const int row = t.row0 + sub * 16 + rr;
     if (parts <= 1 || row >= t.n_rows) return;
     const int tok = t.first_row + row / a.group, qh = head * a.group + row % a.group;
-    const size_t rows = (size_t)a.max_tokens * a.hq, at = (size_t)tok * a.hq + qh;
-    const float2* ml = reinterpret_cast<const float2*>(a.ws + a.splits_max * rows * D) + at;
+    const size_t rows = (size_t)a.max_tokens * a.hq, line = (size_t)tok * a.hq + qh;
+    const float2* ml = reinterpret_cast<const float2*>(a.ws + a.splits_max * rows * D) + line;
     float top = -__builtin_inff(), total = 0.0f, r[8] = {};
     for (int s = 0; s < parts; s++) top = fmaxf(top, ml[s * rows].x);
     for (int s = 0; s < parts; s++) {
         const float2 e = ml[s * rows];
         const float f = e.x == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(e.x - top);
         total += f * e.y;
-        const float4* src = reinterpret_cast<const float4*>(a.ws + (s * rows + at) * D + c8 * 8);
+        const float4* src = reinterpret_cast<const float4*>(a.ws + (s * rows + line) * D + c8 * 8);
         const float4 u = src[0], w = src[1];
         r[0] += f * u.x;
         r[1] += f * u.y;
@@ -1101,8 +1106,12 @@ static void shape_rows(AttnArgs& a, int d)
     set_parts(a, most, want, 1);
 }
 
-// Rows of a request up to which the sixteen-row tiles take it.
-constexpr int kFewRows = 64;
+// Rows of a request up to which the sixteen-row tiles take it.  Over 3000
+// positions each, sixteen-row against 128-row tiles: 8 requests of 64 rows of
+// 36 kv heads 79.7 and 57.9 us, 32 of 64 rows of 8 kv heads 87.8 and 82.1; of
+// 32 rows of 4 kv heads 26.8 and 31.4, 2 of 40 rows of 32 kv heads 25.4 and
+// 28.7.
+constexpr int kFewRows = 48;
 
 // One call's launches: each kernel's arguments, those without tiles left out.
 struct AttnPlan {
