@@ -1028,22 +1028,38 @@ __device__ __forceinline__ void join_parts(const AttnArgs& a, int b)
     const int tok = t.first_row + row / a.group, qh = head * a.group + row % a.group;
     const size_t rows = (size_t)a.max_tokens * a.hq, line = (size_t)tok * a.hq + qh;
     const float2* ml = reinterpret_cast<const float2*>(a.ws + a.splits_max * rows * D) + line;
+    const float* const sums = a.ws + line * D + c8 * 8;
     float top = -__builtin_inff(), total = 0.0f, r[8] = {};
-    for (int s = 0; s < parts; s++) top = fmaxf(top, ml[s * rows].x);
-    for (int s = 0; s < parts; s++) {
-        const float2 e = ml[s * rows];
-        const float f = e.x == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(e.x - top);
-        total += f * e.y;
-        const float4* src = reinterpret_cast<const float4*>(a.ws + (s * rows + line) * D + c8 * 8);
-        const float4 u = src[0], w = src[1];
-        r[0] += f * u.x;
-        r[1] += f * u.y;
-        r[2] += f * u.z;
-        r[3] += f * u.w;
-        r[4] += f * w.x;
-        r[5] += f * w.y;
-        r[6] += f * w.z;
-        r[7] += f * w.w;
+    // several parts' loads in flight: one after the other, a part took the
+    // memory's latency
+    constexpr int kAhead = 8;
+    for (int s0 = 0; s0 < parts; s0 += kAhead) {
+        float2 e[kAhead];
+        float4 u[kAhead][2];
+#pragma unroll
+        for (int i = 0; i < kAhead; i++) {
+            const int s = min(s0 + i, parts - 1);
+            e[i] = ml[s * rows];
+            u[i][0] = *reinterpret_cast<const float4*>(sums + s * rows * D);
+            u[i][1] = *reinterpret_cast<const float4*>(sums + s * rows * D + 4);
+        }
+        float best = top;
+#pragma unroll
+        for (int i = 0; i < kAhead; i++) best = fmaxf(best, e[i].x);
+        const float keep = top == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(top - best);
+        top = best;
+        total *= keep;
+#pragma unroll
+        for (int j = 0; j < 8; j++) r[j] *= keep;
+#pragma unroll
+        for (int i = 0; i < kAhead; i++) {
+            if (s0 + i >= parts || e[i].x == -__builtin_inff()) continue;
+            const float f = __builtin_amdgcn_exp2f(e[i].x - top);
+            const float w[8] = {u[i][0].x, u[i][0].y, u[i][0].z, u[i][0].w, u[i][1].x, u[i][1].y, u[i][1].z, u[i][1].w};
+            total += f * e[i].y;
+#pragma unroll
+            for (int j = 0; j < 8; j++) r[j] += f * w[j];
+        }
     }
     const float inv = total != 0.0f ? 1.0f / total : 0.0f;
 #pragma unroll
