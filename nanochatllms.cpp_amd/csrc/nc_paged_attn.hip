@@ -1108,7 +1108,11 @@ static void shape16(AttnArgs& a)
     const long long tiles = (long long)a.n_req * a.row_tiles * a.hkv, most = most_steps(a, 16, 32);
     long long want = tiles > 0 ? (1024 + tiles - 1) / tiles : 1;
     if (want > (most + 3) / 4) want = (most + 3) / 4;  // a step for each wavefront
-    const long long by_len = (most + 31) / 32;         // 1024 positions
+    // With workgroups enough, parts of 4096 positions even out ragged lengths
+    // (64 requests of up to 8000, 8 kv heads of 128, parts of 1024, 2048 and
+    // 4096: 264, 239 and 232 us; 40 of up to 3900, 36 kv heads, Q8: 124, 116
+    // and 105).
+    const long long by_len = (most + 127) / 128;
     if (want < by_len && tiles < 65536) want = by_len;
     set_parts(a, most, want, 4);
 }
