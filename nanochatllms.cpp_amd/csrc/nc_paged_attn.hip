@@ -202,8 +202,10 @@ __device__ __forceinline__ f32x4 mfma16(half8 a, half8 b, f32x4 c)
 // next step's K is requested as soon as this step's is used up, and so its V:
 // the same registers are always in flight or in use.
 //
-// A Q8 value is its code times its delta, 18 bits: here it enters as two
-// fp16 halves, so a Q8 cache adds no rounding of its own.
+// A Q8 value is its code times its delta, 18 bits, and a probability 24: here
+// both enter as two fp16 halves (of the products of two low halves nothing is
+// left), so the sums are as good as fp32 ones.  These tiles wait for memory,
+// not for the matrix cores.
 
 __device__ __forceinline__ bool pair_not_finite(uint32_t w)
 {
@@ -441,10 +443,16 @@ __device__ __forceinline__ void attn16(const AttnArgs& a, int b, Shared16<D>& sh
         const float m_new = fmaxf(m, mx);
         const float base = m_new == -__builtin_inff() ? 0.0f : m_new - kPScale;
         const float alpha = __builtin_amdgcn_exp2f(m - kPScale - base);
-        half8 p;
+        half8 p, p_lo;
+        float add = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 8; j++) p[j] = (_Float16)__builtin_amdgcn_exp2f(x[j] - base);
-        sum = sum8(p, sum * alpha);
+        for (int j = 0; j < 8; j++) {
+            const float e = __builtin_amdgcn_exp2f(x[j] - base);
+            add += e;
+            p[j] = (_Float16)e;
+            p_lo[j] = (_Float16)(e - (float)p[j]);
+        }
+        sum = __builtin_fmaf(sum, alpha, add);
         m = m_new;
         if (__ballot(alpha != 1.0f)) {
 #pragma unroll
@@ -470,7 +478,9 @@ __device__ __forceinline__ void attn16(const AttnArgs& a, int b, Shared16<D>& sh
             for (int j = 0; j < 8; j++) kv.v_pair(j, i, hi[j], lo[j]);
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-                o[2 * i + e] = mfma16(v_operand(hi, e), p, o[2 * i + e]);
+                const half8 f = v_operand(hi, e);
+                o[2 * i + e] = mfma16(f, p, o[2 * i + e]);
+                o[2 * i + e] = mfma16(f, p_lo, o[2 * i + e]);
                 if constexpr (CDT == Q8) o[2 * i + e] = mfma16(v_operand(lo, e), p, o[2 * i + e]);
             }
             __builtin_amdgcn_sched_barrier(0);
