@@ -311,3 +311,36 @@ def test_wider_pitches(gpu):
     attend(s, cache, wide, b, 4)
     sync()
     assert torch.equal(a.values(), b.values()) and (b.buf[:, 512:] == 0x3C).all()
+
+
+@pytest.mark.parametrize("d,ckind", [(64, "f16"), (128, "q8")])
+def test_chunks_over_more_positions_than_one_lookup_holds(gpu, d, ckind):
+    """128-row tiles look 16384 positions' pages up at a time; entries in the second lot that are no page, too."""
+    s, cache, q = make([60, 3], [20000, 17000], 64, d, 2, 1, "f16", ckind, seed=16)
+    out = Rows("f16", s.max_tokens, 2 * d)
+    attend(s, cache, q, out, 2)
+    sync()
+    check(s, cache, q, out, 2)
+    hidden = [torch.zeros(s.new[r] + s.past[r], dtype=torch.bool) for r in range(2)]
+    for r in range(2):
+        for j in (3, 259, 260):
+            s.table[r, j] = -1
+            hidden[r][j * 64:(j + 1) * 64] = True
+    attend(s, cache, q, out, 2)
+    sync()
+    check(s, cache, q, out, 2, hidden=hidden)
+
+
+@pytest.mark.parametrize("n_req", [65, 150, 700])
+def test_many_requests(gpu, n_req):
+    """Single tokens, chunks and idle requests side by side, more than one probe of a wavefront finds."""
+    g = torch.Generator().manual_seed(n_req)
+    new = (torch.randint(0, 70, (n_req,), generator=g) * (torch.rand(n_req, generator=g) < 0.3)).tolist()
+    new = [n if n or i % 3 else 1 for i, n in enumerate(new)]
+    past = torch.randint(0, 40, (n_req,), generator=g).tolist()
+    for hq, hkv, rows in ((2, 1, "f16"), (1, 1, "q8")):
+        s, cache, q = make(new, past, 16, 64, hq, hkv, rows, rows, seed=n_req)
+        out = Rows(rows, s.max_tokens, hq * 64)
+        attend(s, cache, q, out, hq)
+        sync()
+        check(s, cache, q, out, hq)
