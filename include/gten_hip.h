@@ -270,9 +270,9 @@ int nc_paged_commit(const nc_page_pool* pool, const nc_paged_batch* batch, const
  * nc_rope_table's pairs [rope_rows][d_half]; rope = NULL: no rotation), and
  * stores q to q_out and k and v to the cache at batch->slots.  q, k and v:
  * [max_tokens] rows of one activation dtype; q_out: NC_F16 or NC_Q8, and q
- * itself if of its dtype; q and q_out may both be NULL.  Rows whose slot lies
- * outside the cache or whose position lies outside the rope table are passed
- * over. */
+ * itself if of its dtype, never over k or v; q and q_out may both be NULL.
+ * Rows whose slot lies outside the cache or whose position lies outside the
+ * rope table are passed over. */
 int nc_paged_append(const nc_tensor* q, const nc_tensor* k, const nc_tensor* v, nc_tensor* q_out,
                     const nc_paged_cache* cache, const nc_paged_batch* batch, const float* rope, int rope_rows,
                     int d_half, void* stream);
@@ -283,10 +283,12 @@ int nc_paged_append(const nc_tensor* q, const nc_tensor* k, const nc_tensor* v, 
  * p - window and those below n_sink; 0: all up to its own.  Only pages that
  * hold a visible position are read; positions on an entry that is no page are
  * not seen, and a row that sees nothing is 0.  What lies in unseen positions
- * (NaN too) has no effect.  q and out: rows of NC_F16 or NC_Q8.  Unlike
- * nc_qkv_attn it is not bit for bit the reference's: products on the matrix
- * cores with fp16 factors, statistics and sums in fp32, summed in an order
- * that depends on sizes and lengths alone.  workspace: at least
+ * (NaN too) has no effect.  q and out: rows of NC_F16 or NC_Q8; out may be q
+ * itself (its data, dtype and pitch) and may not lie over it otherwise.
+ * Unlike nc_qkv_attn it is not bit for bit the reference's: scores,
+ * statistics and sums in fp32, in an order that depends on sizes and lengths
+ * alone; of requests with more than 48 new rows (heads of a group counted)
+ * the probabilities and the Q8 values enter rounded to fp16.  workspace: at least
  * nc_paged_attn_workspace's bytes of device memory (16-byte aligned), which
  * calls that may overlap must not share; its contents need no preparation. */
 int nc_paged_attn(const nc_tensor* q, const nc_paged_cache* cache, const nc_paged_batch* batch, nc_tensor* out,
@@ -312,7 +314,8 @@ typedef struct nc_lora {
 /* out = base + scale (x a^T) b^T for each request's rows, with its adapter
  * (adapter[r], [n_req]; one that is no adapter, as -1: out = base).  x: rows
  * of NC_F16 or NC_Q8, k wide; base: fp32 rows, n wide, as nc_matmul_2d leaves
- * them with an fp32 output; out: NC_F32 (base itself too), NC_F16 or NC_Q8.
+ * them with an fp32 output; out: NC_F32 (base itself too), NC_F16 or NC_Q8,
+ * not over x nor otherwise over base.
  * Requests' rows are [row_start[r], row_start[r + 1]), at most max_new each
  * (further ones are left as they were).  Sums in fp32. */
 int nc_lora_add(const nc_tensor* x, const nc_tensor* base, const nc_lora* lora, const int32_t* adapter,

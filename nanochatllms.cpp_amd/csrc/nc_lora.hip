@@ -40,7 +40,7 @@ struct LoraArgs {
 // row's number so that neither side meets in a bank.  No barrier: a
 // wavefront's accesses to it keep their order.
 __device__ __forceinline__ int place16(int row, int piece) { return (row * 16 + (piece ^ row)) * 16; }  // of 256 B rows
-__device__ __forceinline__ int place8(int row, int piece) { return (row * 8 + (piece ^ (row >> 1 & 7))) * 16; }  // of 128 B
+__device__ __forceinline__ int place8(int row, int piece) { return (row * 8 + (piece ^ (row >> 1 & 7))) * 16; }  // 128 B
 
 // Piece of a row of RT * 32 bytes.
 template <int RT>
@@ -51,7 +51,8 @@ __device__ __forceinline__ int place_b(int row, int piece)
 
 // 128 of k (from k0) of sixteen rows of a: lane l loads sixteen bytes of rows
 // l / 16 + 4 i; rows past the rank repeat the last, and b has nothing for them.
-__device__ __forceinline__ void load_a(const LoraArgs& a, const uint16_t* wa, int rank0, int k0, int lane, uint4 (&v)[4])
+__device__ __forceinline__ void load_a(const LoraArgs& a, const uint16_t* wa, int rank0, int k0, int lane,
+                                       uint4 (&v)[4])
 {
     const int k = k0 + lane % 16 * 8;
 #pragma unroll
@@ -258,7 +259,12 @@ constexpr int lora_piece(int rt) { return rt == 8 ? 8192 : 4096; }  // bytes of 
 // One workgroup for sixteen rows and `chunk` columns.  Its wavefronts share
 // out k by 128s, and sum t in shared memory; then each takes 64 columns at a
 // time.  t is made again for every chunk, so chunks are few and workgroups
-// large.
+// large: 16 wavefronts, but 8 from rank 33 on, where 16 leave too few
+// registers (116 to 188 bytes of scratch a lane; 68 and 48 us for 1926 Q8 rows
+// of rank 64, 2304 by 5760, before the pieces' places were spread over the
+// banks, 37 after).  That case moves 99 MB, base and result most of them, at
+// 2.6 TB/s: a workgroup makes t and stores its columns in turn.  32 rows of
+// 32 requests, rank 16, 2048 by 2560: 6 us, three dependent reads' latency.
 template <int XDT, int ODT, int RT>
 __global__ __launch_bounds__(64 * lora_waves(RT)) void k_lora(LoraArgs a)
 {
@@ -420,6 +426,10 @@ extern "C" int nc_lora_add(const nc_tensor* x, const nc_tensor* base, const nc_l
     NC_CHECK_ARG(paged_rows_ok(base, rows, lora->n) && base->dtype == NC_F32,
                  "lora_add: base is not %d aligned fp32 rows of %d values", rows, lora->n);
     NC_CHECK_ARG(paged_rows_ok(out, rows, lora->n), "lora_add: out is not %d aligned rows of %d values", rows, lora->n);
+    // every workgroup of sixteen rows reads all of their x
+    NC_CHECK_ARG(!rows_overlap(x, out, rows), "lora_add: out lies over x");
+    NC_CHECK_ARG(!rows_overlap(base, out, rows) || same_rows(base, out),
+                 "lora_add: out lies over base but is not base");
     if (rows == 0 || max_new == 0) return NC_OK;
     LoraArgs a{};
     a.x = (const uint8_t*)x->data;
@@ -442,6 +452,8 @@ extern "C" int nc_lora_add(const nc_tensor* x, const nc_tensor* base, const nc_l
     a.max_new = max_new;
     const long long tiles = tile_slots(rows, n_req, 1, 16);
     const long long work = max_new == 1 ? n_req : rows / 16 + 1;  // tiles that hold rows, about
+    // 512 workgroups, two for each compute unit (the 1926 rows above with 128,
+    // 256, 384, 512 and 768: 61, 39.3, 39.4, 37.4 and 45 us)
     long long chunks = 512 / work;
     const int most = 64 * lora_waves(a.rank > 32 ? 8 : 1);
     const long long cap = ((long long)a.n + most - 1) / most;  // few wavefronts without columns

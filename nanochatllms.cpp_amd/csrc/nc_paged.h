@@ -16,6 +16,22 @@ inline bool paged_rows_ok(const nc_tensor* t, int rows, int cols)
            t->pitch >= act_pitch(t->dtype, cols) && (t->pitch & 15) == 0;
 }
 
+// Whether [a, a + an) and [b, b + bn) share a byte.
+inline bool share_bytes(const void* a, size_t an, const void* b, size_t bn)
+{
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y + bn && y < x + an;
+}
+inline bool rows_overlap(const nc_tensor* a, const nc_tensor* b, int rows)
+{
+    return rows > 0 && share_bytes(a->data, (size_t)rows * a->pitch, b->data, (size_t)rows * b->pitch);
+}
+// The same rows: a kernel that reads each value where it writes it may.
+inline bool same_rows(const nc_tensor* a, const nc_tensor* b)
+{
+    return a->data == b->data && a->dtype == b->dtype && a->pitch == b->pitch;
+}
+
 int check_cache(const char* what, const nc_paged_cache* c);
 int check_batch(const char* what, const nc_paged_batch* b, int page_size);
 

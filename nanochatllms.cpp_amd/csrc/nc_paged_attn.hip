@@ -16,10 +16,13 @@
 // operand's slots are permuted alike for both factors, so nothing moves
 // between lanes.
 //
-// Roundings: K, V and Q are fp16, probabilities round to fp16 (2^-11 each;
-// the fp16 result rounds as much), everything else is fp32.  Probabilities are scaled by 2^14
-// so that what falls under fp16's smallest number is below 2^-38 of the
-// maximum's weight.
+// Roundings: scores, statistics and sums are fp32.  What the matrix cores take
+// is fp16: in sixteen-row tiles each factor with more bits as two halves that
+// sum to it, so nothing is lost there; in 128-row tiles probabilities, Q8
+// values and Q8 q rows rounded once (2^-11 each; an fp16 result rounds as
+// much), for there the matrix cores are a bound and a second half would double
+// their work.  Probabilities are scaled by 2^14, so that what falls under
+// fp16's smallest number is below 2^-38 of the maximum's weight.
 #include "nc_act.h"
 #include "nc_paged.h"
 
@@ -48,8 +51,9 @@ struct AttnArgs {
     int row_tiles;  // sixteen-row tiles of a request
     int splits;     // parts of a tile's positions at most
     int part;       // steps of a part
-    int splits_max; // of all the call's launches
-    float* ws;      // [splits_max][max_tokens * hq][d] sums, then as many (maximum, sum) pairs
+    size_t lines;   // rows of a part in the workspace: max_tokens * hq, or
+    bool by_tile;   // sixteen for each (sixteen-row tile, kv head), where those are fewer
+    float* ws;      // [splits][lines][d] sums, then as many (maximum, sum) pairs
 };
 
 // acc + the sum of eight fp16 values, in fp32: a row's weights as they enter
@@ -205,7 +209,12 @@ __device__ __forceinline__ f32x4 mfma16(half8 a, half8 b, f32x4 c)
 // A Q8 value is its code times its delta, 18 bits, and a probability 24: here
 // both enter as two fp16 halves (of the products of two low halves nothing is
 // left), so the sums are as good as fp32 ones.  These tiles wait for memory,
-// not for the matrix cores.
+// not for the matrix cores: one token each of 64 requests of up to 8000
+// positions, 32 heads over 8 kv heads of 128, fp16, 1.1 GB: 233 us, 4.7 TB/s
+// (a large copy reaches 4.8); of 40 requests of up to 3900, 36 kv heads of
+// 64, Q8, 397 MB: 108 us, 3.7 TB/s (turning the codes to fp16 fills the issue
+// slots as well).  One request of 700 positions: 8 us, two launches and the
+// latency of page lookup, K, V and the join.
 
 __device__ __forceinline__ bool pair_not_finite(uint32_t w)
 {
@@ -344,6 +353,7 @@ __device__ __forceinline__ void attn16(const AttnArgs& a, int b, Shared16<D>& sh
     const int c = lane & 15, g = lane >> 4;
     const int part = b % a.splits;
     b /= a.splits;
+    const size_t lines0 = (size_t)b * 16;
     const int head = b % a.hkv;
     b /= a.hkv;
     const int req = b / a.row_tiles;
@@ -376,175 +386,175 @@ __device__ __forceinline__ void attn16(const AttnArgs& a, int b, Shared16<D>& sh
     // does not hide, once more for each token, with the values of all
     // positions that it does not see cleared.
     for (int only = -1;;) {
-    const Seen see(a, t, only);
-    float m = -__builtin_inff(), sum = 0.0f;
-    f32x4 o[kDt];
+        const Seen see(a, t, only);
+        float m = -__builtin_inff(), sum = 0.0f;
+        f32x4 o[kDt];
 #pragma unroll
-    for (int i = 0; i < kDt; i++) o[i] = f32x4{0, 0, 0, 0};
+        for (int i = 0; i < kDt; i++) o[i] = f32x4{0, 0, 0, 0};
 
-    Kv16<D, CDT> kv;
-    const int mask = (1 << a.lps) - 1;
-    auto row_of = [&](int page, int pos) {
-        return (((size_t)max(page, 0) * a.hkv + head) << a.lps) + (pos & mask);
-    };
-    int v = v0 + wave;
-    int pos = 0, p0 = 0, p1 = 0;
-    if (v < v1) {
-        pos = steps.at(v) * 32;
-        p0 = page_at(a, req, pos);
-        p1 = page_at(a, req, pos + 16);
-        kv.load_k(a, 0, row_of(p0, pos), c, g);
-        kv.load_k(a, 1, row_of(p1, pos + 16), c, g);
-        kv.load_v(a, 0, row_of(p0, pos), c, g);
-        kv.load_v(a, 1, row_of(p1, pos + 16), c, g);
-    }
-    while (v < v1) {
-        const int nv = v + 4;
-        int npos = 0, np0 = 0, np1 = 0;
-        if (nv < v1) {
-            npos = steps.at(nv) * 32;
-            np0 = page_at(a, req, npos);
-            np1 = page_at(a, req, npos + 16);
+        Kv16<D, CDT> kv;
+        const int mask = (1 << a.lps) - 1;
+        auto row_of = [&](int page, int pos) {
+            return (((size_t)max(page, 0) * a.hkv + head) << a.lps) + (pos & mask);
+        };
+        int v = v0 + wave;
+        int pos = 0, p0 = 0, p1 = 0;
+        if (v < v1) {
+            pos = steps.at(v) * 32;
+            p0 = page_at(a, req, pos);
+            p1 = page_at(a, req, pos + 16);
+            kv.load_k(a, 0, row_of(p0, pos), c, g);
+            kv.load_k(a, 1, row_of(p1, pos + 16), c, g);
+            kv.load_v(a, 0, row_of(p0, pos), c, g);
+            kv.load_v(a, 1, row_of(p1, pos + 16), c, g);
         }
-        f32x4 s[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
-#pragma unroll
-        for (int ks = 0; ks < kKs; ks++)
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const HalfPair8 k = kv.k_operand(h, ks);
-                s[h] = mfma16(k.hi, q[ks].hi, s[h]);
-                if constexpr (CDT == Q8) s[h] = mfma16(k.lo, q[ks].hi, s[h]);
-                if constexpr (QDT == Q8) s[h] = mfma16(k.hi, q[ks].lo, s[h]);
+        while (v < v1) {
+            const int nv = v + 4;
+            int npos = 0, np0 = 0, np1 = 0;
+            if (nv < v1) {
+                npos = steps.at(nv) * 32;
+                np0 = page_at(a, req, npos);
+                np1 = page_at(a, req, npos + 16);
             }
-        __builtin_amdgcn_sched_barrier(0);
-        if (nv < v1) {
-            kv.load_k(a, 0, row_of(np0, npos), c, g);
-            kv.load_k(a, 1, row_of(np1, npos + 16), c, g);
-        }
-        const int last = t.pos0 + t.tok_hi;
-        const bool all = pos + 31 <= t.pos0 + t.tok_lo && p0 >= 0 && p1 >= 0 &&
-                         (!a.window || pos > last - a.window || pos + 31 < a.sink);
-        float x[8];
+            f32x4 s[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
 #pragma unroll
-        for (int j = 0; j < 8; j++) x[j] = s[j >> 2][j & 3] * a.scale;
-        if (!all) {
+            for (int ks = 0; ks < kKs; ks++)
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const int key = pos + 16 * (j >> 2) + 4 * g + (j & 3);
-                const bool seen = (key <= my_pos) & ((key >= my_lo) | (key < a.sink)) & ((j < 4 ? p0 : p1) >= 0);
-                x[j] = seen ? x[j] : -__builtin_inff();
-            }
-        }
-        float mx = x[0];
-#pragma unroll
-        for (int j = 1; j < 8; j++) mx = fmaxf(mx, x[j]);
-        mx = fmaxf(mx, __shfl_xor(mx, 16));
-        mx = fmaxf(mx, __shfl_xor(mx, 32));
-        const float m_new = fmaxf(m, mx);
-        const float base = m_new == -__builtin_inff() ? 0.0f : m_new - kPScale;
-        const float alpha = __builtin_amdgcn_exp2f(m - kPScale - base);
-        half8 p, p_lo;
-        float add = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const float e = __builtin_amdgcn_exp2f(x[j] - base);
-            add += e;
-            p[j] = (_Float16)e;
-            p_lo[j] = (_Float16)(e - (float)p[j]);
-        }
-        sum = __builtin_fmaf(sum, alpha, add);
-        m = m_new;
-        if (__ballot(alpha != 1.0f)) {
-#pragma unroll
-            for (int i = 0; i < kDt; i++) o[i] *= alpha;
-        }
-        // O^T += V^T P^T; positions that no row of the tile sees are cleared,
-        // for a probability of 0 does not hide an infinity or NaN
-        if (!all) {
-            bool odd = false;
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const int key = pos + 16 * (j >> 2) + 4 * g + (j & 3);
-                const bool seen = (key < see.hi) & ((key >= see.lo) | (key < a.sink)) & ((j < 4 ? p0 : p1) >= 0);
-                kv.v_clear(j, seen ? ~0u : 0u);
-                odd |= kv.v_not_finite(j);
-            }
-            if (odd) odd_sh = 1;
-        }
-#pragma unroll
-        for (int i = 0; i < kDt / 2; i++) {
-            uint32_t hi[8], lo[8];
-#pragma unroll
-            for (int j = 0; j < 8; j++) kv.v_pair(j, i, hi[j], lo[j]);
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const half8 f = v_operand(hi, e);
-                o[2 * i + e] = mfma16(f, p, o[2 * i + e]);
-                o[2 * i + e] = mfma16(f, p_lo, o[2 * i + e]);
-                if constexpr (CDT == Q8) o[2 * i + e] = mfma16(v_operand(lo, e), p, o[2 * i + e]);
-            }
+                for (int h = 0; h < 2; h++) {
+                    const HalfPair8 k = kv.k_operand(h, ks);
+                    s[h] = mfma16(k.hi, q[ks].hi, s[h]);
+                    if constexpr (CDT == Q8) s[h] = mfma16(k.lo, q[ks].hi, s[h]);
+                    if constexpr (QDT == Q8) s[h] = mfma16(k.hi, q[ks].lo, s[h]);
+                }
             __builtin_amdgcn_sched_barrier(0);
+            if (nv < v1) {
+                kv.load_k(a, 0, row_of(np0, npos), c, g);
+                kv.load_k(a, 1, row_of(np1, npos + 16), c, g);
+            }
+            const int last = t.pos0 + t.tok_hi;
+            const bool all = pos + 31 <= t.pos0 + t.tok_lo && p0 >= 0 && p1 >= 0 &&
+                             (!a.window || pos > last - a.window || pos + 31 < a.sink);
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[j] = s[j >> 2][j & 3] * a.scale;
+            if (!all) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const int key = pos + 16 * (j >> 2) + 4 * g + (j & 3);
+                    const bool seen = (key <= my_pos) & ((key >= my_lo) | (key < a.sink)) & ((j < 4 ? p0 : p1) >= 0);
+                    x[j] = seen ? x[j] : -__builtin_inff();
+                }
+            }
+            float mx = x[0];
+#pragma unroll
+            for (int j = 1; j < 8; j++) mx = fmaxf(mx, x[j]);
+            mx = fmaxf(mx, __shfl_xor(mx, 16));
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            const float m_new = fmaxf(m, mx);
+            const float base = m_new == -__builtin_inff() ? 0.0f : m_new - kPScale;
+            const float alpha = __builtin_amdgcn_exp2f(m - kPScale - base);
+            half8 p, p_lo;
+            float add = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float e = __builtin_amdgcn_exp2f(x[j] - base);
+                add += e;
+                p[j] = (_Float16)e;
+                p_lo[j] = (_Float16)(e - (float)p[j]);
+            }
+            sum = __builtin_fmaf(sum, alpha, add);
+            m = m_new;
+            if (__ballot(alpha != 1.0f)) {
+#pragma unroll
+                for (int i = 0; i < kDt; i++) o[i] *= alpha;
+            }
+            // O^T += V^T P^T; positions that no row of the tile sees are cleared,
+            // for a probability of 0 does not hide an infinity or NaN
+            if (!all) {
+                bool odd = false;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const int key = pos + 16 * (j >> 2) + 4 * g + (j & 3);
+                    const bool seen = (key < see.hi) & ((key >= see.lo) | (key < a.sink)) & ((j < 4 ? p0 : p1) >= 0);
+                    kv.v_clear(j, seen ? ~0u : 0u);
+                    odd |= kv.v_not_finite(j);
+                }
+                if (odd) odd_sh = 1;
+            }
+#pragma unroll
+            for (int i = 0; i < kDt / 2; i++) {
+                uint32_t hi[8], lo[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) kv.v_pair(j, i, hi[j], lo[j]);
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const half8 f = v_operand(hi, e);
+                    o[2 * i + e] = mfma16(f, p, o[2 * i + e]);
+                    o[2 * i + e] = mfma16(f, p_lo, o[2 * i + e]);
+                    if constexpr (CDT == Q8) o[2 * i + e] = mfma16(v_operand(lo, e), p, o[2 * i + e]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (nv < v1) {
+                kv.load_v(a, 0, row_of(np0, npos), c, g);
+                kv.load_v(a, 1, row_of(np1, npos + 16), c, g);
+            }
+            v = nv;
+            pos = npos;
+            p0 = np0;
+            p1 = np1;
         }
-        if (nv < v1) {
-            kv.load_v(a, 0, row_of(np0, npos), c, g);
-            kv.load_v(a, 1, row_of(np1, npos + 16), c, g);
-        }
-        v = nv;
-        pos = npos;
-        p0 = np0;
-        p1 = np1;
-    }
-    sum += __shfl_xor(sum, 16);
-    sum += __shfl_xor(sum, 32);
+        sum += __shfl_xor(sum, 16);
+        sum += __shfl_xor(sum, 32);
 
-    // join the wavefronts: lane (c, g) holds row c, values (4 g + i) (d / 16) + dt
+        // join the wavefronts: lane (c, g) holds row c, values (4 g + i) (d / 16) + dt
 #pragma unroll
-    for (int i = 0; i < 4; i++)
+        for (int i = 0; i < 4; i++)
 #pragma unroll
-        for (int dt = 0; dt < kDt; dt++) o_sh[wave][c][(4 * g + i) * kDt + dt] = o[dt][i];
-    if (g == 0) {
-        ml_sh[wave][c][0] = m;
-        ml_sh[wave][c][1] = sum;
-    }
-    __syncthreads();
-    if (only < 0 && odd_sh && t.tok_lo != t.tok_hi) {
-        only = t.tok_lo;
+            for (int dt = 0; dt < kDt; dt++) o_sh[wave][c][(4 * g + i) * kDt + dt] = o[dt][i];
+        if (g == 0) {
+            ml_sh[wave][c][0] = m;
+            ml_sh[wave][c][1] = sum;
+        }
         __syncthreads();
-        continue;
-    }
-    const int rr = tid / (D / 8), c8 = tid % (D / 8);
-    const int row = t.row0 + rr, tok = t.first_row + row / a.group, qh = head * a.group + row % a.group;
-    if (rr < 16 && row < t.n_rows && (only < 0 || only == row / a.group)) {  // whole heads
-    float mw[4], top = -__builtin_inff(), total = 0.0f, r[8] = {};
+        if (only < 0 && odd_sh && t.tok_lo != t.tok_hi) {
+            only = t.tok_lo;
+            __syncthreads();
+            continue;
+        }
+        const int rr = tid / (D / 8), c8 = tid % (D / 8);
+        const int row = t.row0 + rr, tok = t.first_row + row / a.group, qh = head * a.group + row % a.group;
+        if (rr < 16 && row < t.n_rows && (only < 0 || only == row / a.group)) {  // whole heads
+            float mw[4], top = -__builtin_inff(), total = 0.0f, r[8] = {};
 #pragma unroll
-    for (int w = 0; w < 4; w++) top = fmaxf(top, mw[w] = ml_sh[w][rr][0]);
+            for (int w = 0; w < 4; w++) top = fmaxf(top, mw[w] = ml_sh[w][rr][0]);
 #pragma unroll
-    for (int w = 0; w < 4; w++) {
-        const float f = mw[w] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mw[w] - top);
-        total += f * ml_sh[w][rr][1];
+            for (int w = 0; w < 4; w++) {
+                const float f = mw[w] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mw[w] - top);
+                total += f * ml_sh[w][rr][1];
 #pragma unroll
-        for (int i = 0; i < 8; i++) r[i] += f * o_sh[w][rr][c8 * 8 + i];
-    }
-    if (parts == 1) {
-        const float inv = total != 0.0f ? 1.0f / total : 0.0f;
+                for (int i = 0; i < 8; i++) r[i] += f * o_sh[w][rr][c8 * 8 + i];
+            }
+            if (parts == 1) {
+                const float inv = total != 0.0f ? 1.0f / total : 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; i++) r[i] *= inv;
-        store_out<D>(a, tok, qh, c8, r);
-    } else {
-    const size_t rows = (size_t)a.max_tokens * a.hq, at = part * rows + (size_t)tok * a.hq + qh;
-    float4* dst = reinterpret_cast<float4*>(a.ws + at * D + c8 * 8);
-    dst[0] = make_float4(r[0], r[1], r[2], r[3]);
-    dst[1] = make_float4(r[4], r[5], r[6], r[7]);
-    if (c8 == 0) {
-        float* ml = a.ws + a.splits_max * rows * D + at * 2;
-        ml[0] = top;
-        ml[1] = total;
-    }
-    }
-    }
-    if (only < 0 || only == t.tok_hi) return;
-    only++;
-    __syncthreads();
+                for (int i = 0; i < 8; i++) r[i] *= inv;
+                store_out<D>(a, tok, qh, c8, r);
+            } else {
+                const size_t at = part * a.lines + (a.by_tile ? lines0 + rr : (size_t)tok * a.hq + qh);
+                float4* dst = reinterpret_cast<float4*>(a.ws + at * D + c8 * 8);
+                dst[0] = make_float4(r[0], r[1], r[2], r[3]);
+                dst[1] = make_float4(r[4], r[5], r[6], r[7]);
+                if (c8 == 0) {
+                    float* ml = a.ws + a.splits * a.lines * D + at * 2;
+                    ml[0] = top;
+                    ml[1] = total;
+                }
+            }
+        }
+        if (only < 0 || only == t.tok_hi) return;
+        only++;
+        __syncthreads();
     }
 }
 
@@ -569,6 +579,14 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 3) void k_paged_attn16(AttnArgs 
 // row, so that sixteen neighbouring lanes' reads spread over all banks.
 //
 // Q8 values and q rows enter as their fp16 products, rounded once (2^-11).
+//
+// Bound by the instructions issued around the matrix ones (a wavefront issues
+// one every 7 cycles, four on a SIMD one every 3; per step of 64 positions
+// and 32 rows 32 exponentials, as many conversions and 64 scalings and maxima
+// stand against 16 matrix instructions of 33 cycles): 4 chunks of 500 rows
+// over 2000 positions, 32 heads over 4 kv heads of 64, 26 GFLOP: 60 us, 430
+// TFLOP/s; two of 1000 rows under a window of 1024, 8 kv heads of 128, 36
+// GFLOP: 88 us, 410 TFLOP/s.  Sixteen-row tiles took 139 and 248.
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
@@ -771,220 +789,220 @@ __device__ __forceinline__ void attn_rows(const AttnArgs& a, int b, SharedRows<D
     // does not hide, once more for each token, with the values of all
     // positions that it does not see cleared.
     for (int only = -1;;) {
-    const Seen see(a, t, only);
-    float m = -__builtin_inff(), sum = 0.0f;
-    f32x16 o[kDt];
+        const Seen see(a, t, only);
+        float m = -__builtin_inff(), sum = 0.0f;
+        f32x16 o[kDt];
 #pragma unroll
-    for (int i = 0; i < kDt; i++) o[i] = f32x16{};
+        for (int i = 0; i < kDt; i++) o[i] = f32x16{};
 
-    for (int vt = v0; vt < v1; vt += kPlaces / kG) {
-    const int vn = min(v1 - vt, kPlaces / kG);
-    if (vt != v0) __syncthreads();  // the places are read before they are written again
-    if (tid < kPlaces / 32) places.none[tid] = 0;
-    if (tid == 0) places.some_none = 0;
-    __syncthreads();
-    for (int e = tid; e < vn * kG; e += 256) {
-        const int pos = steps.at(vt + e / kG) * kS + e % kG * 16;
-        const int id = a.table[(size_t)req * a.max_pages + min(pos >> a.lps, a.max_pages - 1)];
-        const bool page = (unsigned)id < (unsigned)a.n_pages;
-        const size_t row = (((size_t)(page ? id : 0) * a.hkv + head) << a.lps) + (pos & ((1 << a.lps) - 1));
-        places.at[e] = row * (CDT == Q8 ? D : 2 * D);
-        // sixteens that no row sees are masked by their positions
-        if (!page && pos < t.hi && (pos + 15 >= t.lo || pos < a.sink)) {
-            atomicOr(&places.none[e >> 5], 1u << (e & 31));
-            places.some_none = 1;
-        }
-    }
-    __syncthreads();
-    const bool some_none = places.some_none != 0;
-
-    // Step i computes the scores of step i + 1 between its exponentials, then
-    // multiplies those with its V; K of step i + 2 and V of step i + 1 are on
-    // their way from memory.
-    auto clamped = [&](int i) { return min(i, vn - 1); };
-    auto pos_of = [&](int i) { return steps.at(vt + clamped(i)) * kS; };
-    half8 kf[kKs][kU];
-    auto read_k = [&](const uint8_t* kb) {
-#pragma unroll
-        for (int ks = 0; ks < kKs; ks++)
-#pragma unroll
-            for (int u = 0; u < kU; u++)
-                kf[ks][u] = *reinterpret_cast<const half8*>(kb + k_place<D>(u * 32 + c, ks * 2 + h));
-    };
-    // whether all rows from token lo to hi see the whole step at pos
-    auto all_see = [&](int pos, int lo, int hi) {
-        return !some_none & (pos + kS - 1 <= t.pos0 + lo) &
-               ((a.window == 0) | (pos > t.pos0 + hi - a.window) | (pos + kS - 1 < a.sink));
-    };
-    // places of the next loads, read a step ahead
-    unsigned long long k_at0, k_at1, v_at;
-    auto places_of = [&](int ik, int iv) {
-        const unsigned long long* p = places.at + clamped(ik) * kG;
-        k_at0 = p[KvRows<D, CDT>::k_sixteen(0, wave)];
-        k_at1 = p[KvRows<D, CDT>::k_sixteen(1, wave)];
-        v_at = places.at[clamped(iv) * kG + KvRows<D, CDT>::v_sixteen(wave)];
-    };
-    auto store_v = [&](const KvRows<D, CDT>& from, uint8_t* vb, int i) {
-        const int pos = pos_of(i), e = clamped(i) * kG + KvRows<D, CDT>::v_sixteen(wave);
-        const bool page = !some_none || !((places.none[e >> 5] >> (e & 31)) & 1);
-        from.store_v(vb, a, see, !all_see(pos, t.tok_lo, t.tok_hi), pos, page, &odd_sh);
-    };
-    KvRows<D, CDT> kv;
-    f32x16 s[kU], t_s[kU];
-    {
-        KvRows<D, CDT> w;
-        places_of(0, 0);
-        kv.load_k(a, k_at0, k_at1, wave);
-        kv.load_v(a, v_at, wave);
-        places_of(1, 1);
-        w.load_k(a, k_at0, k_at1, wave);
-        places_of(2, 1);
-        kv.store_k(k_sh[0]);
-        store_v(kv, v_sh[0], 0);
-        w.store_k(k_sh[1]);
-    }
-    __syncthreads();
-    read_k(k_sh[0]);
-#pragma unroll
-    for (int u = 0; u < kU; u++) s[u] = t_s[u] = f32x16{};
-#pragma unroll
-    for (int ks = 0; ks < kKs; ks++)
-#pragma unroll
-        for (int u = 0; u < kU; u++) s[u] = mfma32(kf[ks][u], q[ks], s[u]);
-    __syncthreads();
-    auto step = [&](f32x16 (&s)[kU], f32x16 (&s_next)[kU], int i0, int buf) {
-        if (i0 + 2 < vn) kv.load_k(a, k_at0, k_at1, wave);
-        if (i0 + 1 < vn) kv.load_v(a, v_at, wave);
-        places_of(i0 + 3, i0 + 2);
-        const int pos = pos_of(i0);
-        // unless the wavefront sees none of the step's positions
-        if (mine && pos <= t.pos0 + w_hi) {
-            const uint8_t* vb = v_sh[buf];
-            auto read_v = [&](int i) {  // operand i: values 32 (i % kDt) of sixteen i / kDt
-                return *reinterpret_cast<const half8*>(vb + v_place<D>(i % kDt * 32 + c, i / kDt * 2 + h));
-            };
-            constexpr int kNv = 2 * kU * kDt, kAhead = D == 128 ? 4 : 8;
-            read_k(k_sh[buf ^ 1]);
-            if (!all_see(pos, w_lo, w_hi)) {
-                // against the lane's first position: its others lie at constants
-                const int at0 = pos + 4 * h, hi = my_pos - at0, lo = my_lo - at0, sk = a.sink - at0;
-                int none = 0;
-                if (some_none) none = places.none[clamped(i0) * kG >> 5] >> (clamped(i0) * kG & 31);
-#pragma unroll
-                for (int i = 0; i < 16 * kU; i++) {
-                    const int at = (i >> 4) * 32 + ((i >> 2) & 3) * 8 + (i & 3);
-                    const bool seen = (at <= hi) & ((at >= lo) | (at < sk)) & !((none >> (at >> 4)) & 1);
-                    s[i >> 4][i & 15] = seen ? s[i >> 4][i & 15] : -__builtin_inff();
+        for (int vt = v0; vt < v1; vt += kPlaces / kG) {
+            const int vn = min(v1 - vt, kPlaces / kG);
+            if (vt != v0) __syncthreads();  // the places are read before they are written again
+            if (tid < kPlaces / 32) places.none[tid] = 0;
+            if (tid == 0) places.some_none = 0;
+            __syncthreads();
+            for (int e = tid; e < vn * kG; e += 256) {
+                const int pos = steps.at(vt + e / kG) * kS + e % kG * 16;
+                const int id = a.table[(size_t)req * a.max_pages + min(pos >> a.lps, a.max_pages - 1)];
+                const bool page = (unsigned)id < (unsigned)a.n_pages;
+                const size_t row = (((size_t)(page ? id : 0) * a.hkv + head) << a.lps) + (pos & ((1 << a.lps) - 1));
+                places.at[e] = row * (CDT == Q8 ? D : 2 * D);
+                // sixteens that no row sees are masked by their positions
+                if (!page && pos < t.hi && (pos + 15 >= t.lo || pos < a.sink)) {
+                    atomicOr(&places.none[e >> 5], 1u << (e & 31));
+                    places.some_none = 1;
                 }
             }
-            float mx = s[0][0];
-#pragma unroll
-            for (int i = 1; i < 16 * kU; i++) mx = fmaxf(mx, s[i >> 4][i & 15]);
-            mx = fmaxf(mx, __shfl_xor(mx, 32)) * a.scale;
-            // the reference point follows the maximum once it is 2^kPSlack
-            // behind: most steps leave the sums as they are
-            if (__ballot(mx > m + kPSlack)) {
-                const float m_new = fmaxf(m, mx);
-                const float alpha = __builtin_amdgcn_exp2f(m_new == -__builtin_inff() ? 0.0f : m - m_new);
-                sum *= alpha;
-#pragma unroll
-                for (int i = 0; i < kDt; i++) o[i] *= alpha;
-                m = m_new;
-            }
-            const float base = m == -__builtin_inff() ? 0.0f : m - (kPScale - kPSlack);
-            // Each matrix instruction of the next step's scores between some
-            // of this step's exponentials: in a run of their own each kind
-            // leaves the other's unit idle, in step with the other wavefronts.
-            half8 p[2 * kU], vf[kAhead];
-#pragma unroll
-            for (int i = 0; i < kAhead; i++) vf[i] = read_v(i);
-            constexpr int kN = kKs * kU, kEach = 16 * kU / kN;
-#pragma unroll
-            for (int u = 0; u < kU; u++) s_next[u] = f32x16{};
-#pragma unroll
-            for (int n = 0; n < kN; n++) {
-                s_next[n % kU] = mfma32(kf[n / kU][n % kU], q[n / kU], s_next[n % kU]);
-#pragma unroll
-                for (int i = n * kEach; i < (n + 1) * kEach; i++)
-                    p[i >> 3][i & 7] =
-                        (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 4][i & 15], a.scale, -base));
-                __builtin_amdgcn_sched_barrier(0);
-            }
-#pragma unroll
-            for (int i = 0; i < kNv; i++) {
-                const half8 f = vf[i % kAhead];
-                if (i + kAhead < kNv) vf[i % kAhead] = read_v(i + kAhead);
-                o[i % kDt] = mfma32(f, p[i / kDt], o[i % kDt]);
-                if (i % kDt == kDt - 1) sum = sum8(p[i / kDt], sum);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-        }
-        // what these overwrite was last read before the last barrier
-        if (i0 + 2 < vn) kv.store_k(k_sh[buf]);
-        if (i0 + 1 < vn) store_v(kv, v_sh[buf ^ 1], i0 + 1);
-        __syncthreads();
-    };
-    for (int i0 = 0; i0 < vn; i0 += 2) {
-        step(s, t_s, i0, 0);
-        if (i0 + 1 < vn) step(t_s, s, i0 + 1, 1);
-    }
-    }
-    sum += __shfl_xor(sum, 32);
-    if (only < 0 && odd_sh && t.tok_lo != t.tok_hi) {
-        only = t.tok_lo;
-        __syncthreads();  // odd_sh is read before it is written again
-        continue;
-    }
-    if (first + c < t.n_rows && (only < 0 || only == my_tok)) {
+            __syncthreads();
+            const bool some_none = places.some_none != 0;
 
-    // lane (c, h): row c, values 32 dt + 8 j + 4 h + i
-    const int tok = t.first_row + my_tok, qh = head * a.group + my % a.group;
-    if (parts > 1) {
-        const size_t rows = (size_t)a.max_tokens * a.hq, at = part * rows + (size_t)tok * a.hq + qh;
+            // Step i computes the scores of step i + 1 between its exponentials, then
+            // multiplies those with its V; K of step i + 2 and V of step i + 1 are on
+            // their way from memory.
+            auto clamped = [&](int i) { return min(i, vn - 1); };
+            auto pos_of = [&](int i) { return steps.at(vt + clamped(i)) * kS; };
+            half8 kf[kKs][kU];
+            auto read_k = [&](const uint8_t* kb) {
 #pragma unroll
-        for (int dt = 0; dt < kDt; dt++)
+                for (int ks = 0; ks < kKs; ks++)
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                *reinterpret_cast<float4*>(a.ws + at * D + dt * 32 + j * 8 + h * 4) =
-                    make_float4(o[dt][4 * j], o[dt][4 * j + 1], o[dt][4 * j + 2], o[dt][4 * j + 3]);
-        if (h == 0) *reinterpret_cast<float2*>(a.ws + a.splits_max * rows * D + at * 2) = make_float2(m, sum);
-    } else {
-    const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
-    uint8_t* op = a.out + (size_t)tok * a.out_pitch;
-#pragma unroll
-    for (int dt = 0; dt < kDt; dt++) {
-        if (a.out_dtype == F16) {
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                float v[4];
-#pragma unroll
-                for (int i = 0; i < 4; i++) v[i] = o[dt][4 * j + i] * inv;
-                *reinterpret_cast<uint2*>(op + (qh * D + dt * 32 + j * 8 + h * 4) * 2) =
-                    make_uint2((uint32_t)f2h(v[0]) | (uint32_t)f2h(v[1]) << 16,
-                               (uint32_t)f2h(v[2]) | (uint32_t)f2h(v[3]) << 16);
+                    for (int u = 0; u < kU; u++)
+                        kf[ks][u] = *reinterpret_cast<const half8*>(kb + k_place<D>(u * 32 + c, ks * 2 + h));
+            };
+            // whether all rows from token lo to hi see the whole step at pos
+            auto all_see = [&](int pos, int lo, int hi) {
+                return !some_none & (pos + kS - 1 <= t.pos0 + lo) &
+                       ((a.window == 0) | (pos > t.pos0 + hi - a.window) | (pos + kS - 1 < a.sink));
+            };
+            // places of the next loads, read a step ahead
+            unsigned long long k_at0, k_at1, v_at;
+            auto places_of = [&](int ik, int iv) {
+                const unsigned long long* p = places.at + clamped(ik) * kG;
+                k_at0 = p[KvRows<D, CDT>::k_sixteen(0, wave)];
+                k_at1 = p[KvRows<D, CDT>::k_sixteen(1, wave)];
+                v_at = places.at[clamped(iv) * kG + KvRows<D, CDT>::v_sixteen(wave)];
+            };
+            auto store_v = [&](const KvRows<D, CDT>& from, uint8_t* vb, int i) {
+                const int pos = pos_of(i), e = clamped(i) * kG + KvRows<D, CDT>::v_sixteen(wave);
+                const bool page = !some_none || !((places.none[e >> 5] >> (e & 31)) & 1);
+                from.store_v(vb, a, see, !all_see(pos, t.tok_lo, t.tok_hi), pos, page, &odd_sh);
+            };
+            KvRows<D, CDT> kv;
+            f32x16 s[kU], t_s[kU];
+            {
+                KvRows<D, CDT> w;
+                places_of(0, 0);
+                kv.load_k(a, k_at0, k_at1, wave);
+                kv.load_v(a, v_at, wave);
+                places_of(1, 1);
+                w.load_k(a, k_at0, k_at1, wave);
+                places_of(2, 1);
+                kv.store_k(k_sh[0]);
+                store_v(kv, v_sh[0], 0);
+                w.store_k(k_sh[1]);
             }
-        } else {
-            // q8_quantize of a block whose halves two lanes hold
-            float top = 0.0f;
+            __syncthreads();
+            read_k(k_sh[0]);
 #pragma unroll
-            for (int i = 0; i < 16; i++) top = fmaxf(top, fabsf(o[dt][i] * inv));
-            top = fmaxf(top, __shfl_xor(top, 32));
-            const float delta = top / 127.0f, by = delta != 0.0f ? 1.0f / delta : 0.0f;
+            for (int u = 0; u < kU; u++) s[u] = t_s[u] = f32x16{};
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                uint32_t w = 0;
+            for (int ks = 0; ks < kKs; ks++)
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    w |= (uint32_t)(uint8_t)(int8_t)roundf(o[dt][4 * j + i] * inv * by) << (8 * i);
-                *reinterpret_cast<uint32_t*>(op + qh * D + dt * 32 + j * 8 + h * 4) = w;
+                for (int u = 0; u < kU; u++) s[u] = mfma32(kf[ks][u], q[ks], s[u]);
+            __syncthreads();
+            auto step = [&](f32x16 (&s)[kU], f32x16 (&s_next)[kU], int i0, int buf) {
+                if (i0 + 2 < vn) kv.load_k(a, k_at0, k_at1, wave);
+                if (i0 + 1 < vn) kv.load_v(a, v_at, wave);
+                places_of(i0 + 3, i0 + 2);
+                const int pos = pos_of(i0);
+                // unless the wavefront sees none of the step's positions
+                if (mine && pos <= t.pos0 + w_hi) {
+                    const uint8_t* vb = v_sh[buf];
+                    auto read_v = [&](int i) {  // operand i: values 32 (i % kDt) of sixteen i / kDt
+                        return *reinterpret_cast<const half8*>(vb + v_place<D>(i % kDt * 32 + c, i / kDt * 2 + h));
+                    };
+                    constexpr int kNv = 2 * kU * kDt, kAhead = D == 128 ? 4 : 8;
+                    read_k(k_sh[buf ^ 1]);
+                    if (!all_see(pos, w_lo, w_hi)) {
+                        // against the lane's first position: its others lie at constants
+                        const int at0 = pos + 4 * h, hi = my_pos - at0, lo = my_lo - at0, sk = a.sink - at0;
+                        int none = 0;
+                        if (some_none) none = places.none[clamped(i0) * kG >> 5] >> (clamped(i0) * kG & 31);
+#pragma unroll
+                        for (int i = 0; i < 16 * kU; i++) {
+                            const int at = (i >> 4) * 32 + ((i >> 2) & 3) * 8 + (i & 3);
+                            const bool seen = (at <= hi) & ((at >= lo) | (at < sk)) & !((none >> (at >> 4)) & 1);
+                            s[i >> 4][i & 15] = seen ? s[i >> 4][i & 15] : -__builtin_inff();
+                        }
+                    }
+                    float mx = s[0][0];
+#pragma unroll
+                    for (int i = 1; i < 16 * kU; i++) mx = fmaxf(mx, s[i >> 4][i & 15]);
+                    mx = fmaxf(mx, __shfl_xor(mx, 32)) * a.scale;
+                    // the reference point follows the maximum once it is 2^kPSlack
+                    // behind: most steps leave the sums as they are
+                    if (__ballot(mx > m + kPSlack)) {
+                        const float m_new = fmaxf(m, mx);
+                        const float alpha = __builtin_amdgcn_exp2f(m_new == -__builtin_inff() ? 0.0f : m - m_new);
+                        sum *= alpha;
+#pragma unroll
+                        for (int i = 0; i < kDt; i++) o[i] *= alpha;
+                        m = m_new;
+                    }
+                    const float base = m == -__builtin_inff() ? 0.0f : m - (kPScale - kPSlack);
+                    // Each matrix instruction of the next step's scores between some
+                    // of this step's exponentials: in a run of their own each kind
+                    // leaves the other's unit idle, in step with the other wavefronts.
+                    half8 p[2 * kU], vf[kAhead];
+#pragma unroll
+                    for (int i = 0; i < kAhead; i++) vf[i] = read_v(i);
+                    constexpr int kN = kKs * kU, kEach = 16 * kU / kN;
+#pragma unroll
+                    for (int u = 0; u < kU; u++) s_next[u] = f32x16{};
+#pragma unroll
+                    for (int n = 0; n < kN; n++) {
+                        s_next[n % kU] = mfma32(kf[n / kU][n % kU], q[n / kU], s_next[n % kU]);
+#pragma unroll
+                        for (int i = n * kEach; i < (n + 1) * kEach; i++)
+                            p[i >> 3][i & 7] =
+                                (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 4][i & 15], a.scale, -base));
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+#pragma unroll
+                    for (int i = 0; i < kNv; i++) {
+                        const half8 f = vf[i % kAhead];
+                        if (i + kAhead < kNv) vf[i % kAhead] = read_v(i + kAhead);
+                        o[i % kDt] = mfma32(f, p[i / kDt], o[i % kDt]);
+                        if (i % kDt == kDt - 1) sum = sum8(p[i / kDt], sum);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
+                // what these overwrite was last read before the last barrier
+                if (i0 + 2 < vn) kv.store_k(k_sh[buf]);
+                if (i0 + 1 < vn) store_v(kv, v_sh[buf ^ 1], i0 + 1);
+                __syncthreads();
+            };
+            for (int i0 = 0; i0 < vn; i0 += 2) {
+                step(s, t_s, i0, 0);
+                if (i0 + 1 < vn) step(t_s, s, i0 + 1, 1);
             }
-            if (h == 0) reinterpret_cast<uint16_t*>(op + a.hq * D)[qh * kDt + dt] = f2h(delta);
         }
-    }
-    }
-    }
-    if (only < 0 || only == t.tok_hi) return;
-    only++;
+        sum += __shfl_xor(sum, 32);
+        if (only < 0 && odd_sh && t.tok_lo != t.tok_hi) {
+            only = t.tok_lo;
+            __syncthreads();  // odd_sh is read before it is written again
+            continue;
+        }
+        if (first + c < t.n_rows && (only < 0 || only == my_tok)) {
+
+            // lane (c, h): row c, values 32 dt + 8 j + 4 h + i
+            const int tok = t.first_row + my_tok, qh = head * a.group + my % a.group;
+            if (parts > 1) {
+                const size_t at = part * a.lines + (size_t)tok * a.hq + qh;
+#pragma unroll
+                for (int dt = 0; dt < kDt; dt++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        *reinterpret_cast<float4*>(a.ws + at * D + dt * 32 + j * 8 + h * 4) =
+                            make_float4(o[dt][4 * j], o[dt][4 * j + 1], o[dt][4 * j + 2], o[dt][4 * j + 3]);
+                if (h == 0) *reinterpret_cast<float2*>(a.ws + a.splits * a.lines * D + at * 2) = make_float2(m, sum);
+            } else {
+                const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+                uint8_t* op = a.out + (size_t)tok * a.out_pitch;
+#pragma unroll
+                for (int dt = 0; dt < kDt; dt++) {
+                    if (a.out_dtype == F16) {
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            float v[4];
+#pragma unroll
+                            for (int i = 0; i < 4; i++) v[i] = o[dt][4 * j + i] * inv;
+                            *reinterpret_cast<uint2*>(op + (qh * D + dt * 32 + j * 8 + h * 4) * 2) =
+                                make_uint2((uint32_t)f2h(v[0]) | (uint32_t)f2h(v[1]) << 16,
+                                           (uint32_t)f2h(v[2]) | (uint32_t)f2h(v[3]) << 16);
+                        }
+                    } else {
+                        // q8_quantize of a block whose halves two lanes hold
+                        float top = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < 16; i++) top = fmaxf(top, fabsf(o[dt][i] * inv));
+                        top = fmaxf(top, __shfl_xor(top, 32));
+                        const float delta = top / 127.0f, by = delta != 0.0f ? 1.0f / delta : 0.0f;
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            uint32_t w = 0;
+#pragma unroll
+                            for (int i = 0; i < 4; i++)
+                                w |= (uint32_t)(uint8_t)(int8_t)roundf(o[dt][4 * j + i] * inv * by) << (8 * i);
+                            *reinterpret_cast<uint32_t*>(op + qh * D + dt * 32 + j * 8 + h * 4) = w;
+                        }
+                        if (h == 0) reinterpret_cast<uint16_t*>(op + a.hq * D)[qh * kDt + dt] = f2h(delta);
+                    }
+                }
+            }
+        }
+        if (only < 0 || only == t.tok_hi) return;
+        only++;
     }
 }
 
@@ -1008,10 +1026,13 @@ __global__ __launch_bounds__(256, 2) void k_paged_mixed(MixedArgs a)
 // ---- parts joined ----------------------------------------------------------------
 
 // A row's parts in their order, sixteen rows a workgroup: the rows of tiles of
-// M rows that visit their positions in steps of S.
+// M rows that visit their positions in steps of S.  A launch of its own:
+// counting parts down in the last to end would need counters that a caller
+// keeps clear.  Bound by two dependent reads' latency, 3 to 4 us.
 template <int D, int M, int S>
 __device__ __forceinline__ void join_parts(const AttnArgs& a, int b)
 {
+    const size_t lines0 = (size_t)b * 16;
     const int head = b % a.hkv;
     b /= a.hkv;
     Tile t;
@@ -1036,8 +1057,8 @@ __device__ __forceinline__ void join_parts(const AttnArgs& a, int b)
     const int row = t.row0 + sub * 16 + rr;
     if (parts <= 1 || row >= t.n_rows) return;
     const int tok = t.first_row + row / a.group, qh = head * a.group + row % a.group;
-    const size_t rows = (size_t)a.max_tokens * a.hq, line = (size_t)tok * a.hq + qh;
-    const float2* ml = reinterpret_cast<const float2*>(a.ws + a.splits_max * rows * D) + line;
+    const size_t line = M == 16 && a.by_tile ? lines0 + rr : (size_t)tok * a.hq + qh;
+    const float2* ml = reinterpret_cast<const float2*>(a.ws + a.splits * a.lines * D) + line;
     const float* const sums = a.ws + line * D + c8 * 8;
     float top = -__builtin_inff(), total = 0.0f, r[8] = {};
     // several parts' loads in flight: one after the other, a part took the
@@ -1049,9 +1070,9 @@ __device__ __forceinline__ void join_parts(const AttnArgs& a, int b)
 #pragma unroll
         for (int i = 0; i < kAhead; i++) {
             const int s = min(s0 + i, parts - 1);
-            e[i] = ml[s * rows];
-            u[i][0] = *reinterpret_cast<const float4*>(sums + s * rows * D);
-            u[i][1] = *reinterpret_cast<const float4*>(sums + s * rows * D + 4);
+            e[i] = ml[s * a.lines];
+            u[i][0] = *reinterpret_cast<const float4*>(sums + s * a.lines * D);
+            u[i][1] = *reinterpret_cast<const float4*>(sums + s * a.lines * D + 4);
         }
         float best = top;
 #pragma unroll
@@ -1111,18 +1132,23 @@ static void set_parts(AttnArgs& a, long long most, long long want, int unit)
 }
 
 // The tiles of sixteen rows, for requests of at most `few` (token, head) rows.
-static void shape16(AttnArgs& a)
+static void shape16(AttnArgs& a, int d)
 {
     const long long rows = (long long)(a.max_new < a.max_tokens ? a.max_new : a.max_tokens) * a.group;
     a.row_tiles = (int)(((rows < a.few ? rows : a.few) + 15) / 16);
     const long long tiles = (long long)a.n_req * a.row_tiles * a.hkv, most = most_steps(a, 16, 32);
+    const long long by_token = (long long)a.max_tokens * a.hq;
+    a.by_tile = tiles * 16 < by_token;
+    a.lines = (size_t)(a.by_tile ? tiles * 16 : by_token);
     long long want = tiles > 0 ? (1024 + tiles - 1) / tiles : 1;
     if (want > (most + 3) / 4) want = (most + 3) / 4;  // a step for each wavefront
     // With workgroups enough, parts of 4096 positions even out ragged lengths
     // (64 requests of up to 8000, 8 kv heads of 128, parts of 1024, 2048 and
     // 4096: 264, 239 and 232 us; 40 of up to 3900, 36 kv heads, Q8: 124, 116
-    // and 105).
-    const long long by_len = (most + 127) / 128;
+    // and 105), within 1 GB of workspace.
+    long long by_len = (most + 127) / 128;
+    const long long room = a.lines ? (1ll << 30) / ((long long)a.lines * (d + 2) * 4) : 1;
+    if (by_len > room) by_len = room;
     if (want < by_len && tiles < 65536) want = by_len;
     set_parts(a, most, want, 4);
 }
@@ -1130,7 +1156,10 @@ static void shape16(AttnArgs& a)
 // The tiles of 128 rows, for the others.
 static void shape_rows(AttnArgs& a, int d)
 {
-    const long long tiles = ((long long)a.max_tokens * a.group / kRowsM + 1) * a.hkv, most = most_steps(a, kRowsM, rows_step(d));
+    const int S = rows_step(d);
+    const long long tiles = ((long long)a.max_tokens * a.group / kRowsM + 1) * a.hkv, most = most_steps(a, kRowsM, S);
+    a.by_tile = false;
+    a.lines = (size_t)a.max_tokens * a.hq;
     long long want = (512 + tiles - 1) / tiles;
     if (want > (most + 3) / 4) want = (most + 3) / 4;
     set_parts(a, most, want, 1);
@@ -1146,25 +1175,25 @@ constexpr int kFewRows = 48;
 // One call's launches: each kernel's arguments, those without tiles left out.
 struct AttnPlan {
     AttnArgs few, rows;
-    bool some_few, some_rows;
+    bool some_rows;
 };
 static AttnPlan attn_plan(const AttnArgs& base, int d)
 {
-    AttnPlan p{base, base, true, false};
+    AttnPlan p{base, base, false};
     p.few.few = p.rows.few = kFewRows;
     p.some_rows = (long long)(base.max_new < base.max_tokens ? base.max_new : base.max_tokens) * base.group > kFewRows;
-    shape16(p.few);
+    shape16(p.few, d);
     if (p.some_rows) shape_rows(p.rows, d);
-    const int most = p.some_rows && p.rows.splits > p.few.splits ? p.rows.splits : p.few.splits;
-    p.few.splits_max = p.rows.splits_max = most;
     return p;
 }
 
-static size_t attn_ws_bytes(const AttnPlan& p, int d)
+// The workspace: the 128-row tiles' parts, then the sixteen-row tiles'.
+static size_t parts_bytes(const AttnArgs& a, int d)
 {
-    const AttnArgs& a = p.few;
-    return a.splits_max > 1 ? (size_t)a.splits_max * a.max_tokens * a.hq * (d + 2) * 4 : 0;
+    return a.splits > 1 ? ((size_t)a.splits * a.lines * (d + 2) * 4 + 15) / 16 * 16 : 0;
 }
+static size_t rows_ws_bytes(const AttnPlan& p, int d) { return p.some_rows ? parts_bytes(p.rows, d) : 0; }
+static size_t attn_ws_bytes(const AttnPlan& p, int d) { return rows_ws_bytes(p, d) + parts_bytes(p.few, d); }
 
 static int attn_args(AttnArgs& a, const nc_paged_cache* cache, const nc_paged_batch* b, int n_heads, int window,
                      int n_sink)
@@ -1205,12 +1234,12 @@ static int attn_launch(const AttnPlan& p, hipStream_t st)
     const long long slots = tile_slots(r.max_tokens, r.n_req, r.group, kRowsM) * r.hkv;
     NC_CHECK_ARG(tiles * f.splits <= 0xFFFFFF && (!p.some_rows || slots * 8 * r.splits <= 0xFFFFFF),
                  "paged_attn: %lld tiles of %d parts are too many for one launch", tiles > slots ? tiles : slots,
-                 f.splits_max);
+                 p.some_rows && r.splits > f.splits ? r.splits : f.splits);
     if (p.some_rows) {
         MixedArgs m{r, f, (int)(slots * r.splits)};
-        hipLaunchKernelGGL((k_paged_mixed<D, CDT, QDT>), dim3((unsigned)(m.row_blocks + tiles * f.splits)), dim3(256), 0,
-                           st, m);
-        if (f.splits_max > 1) {
+        const unsigned grid = (unsigned)(m.row_blocks + tiles * f.splits);
+        hipLaunchKernelGGL((k_paged_mixed<D, CDT, QDT>), dim3(grid), dim3(256), 0, st, m);
+        if (f.splits > 1 || r.splits > 1) {
             m.row_blocks = r.splits > 1 ? (int)(slots * (kRowsM / 16)) : 0;
             const unsigned blocks = (unsigned)(m.row_blocks + (f.splits > 1 ? tiles : 0));
             hipLaunchKernelGGL((k_paged_join_mixed<D>), dim3(blocks), dim3(16 * D / 8), 0, st, m);
@@ -1253,19 +1282,21 @@ extern "C" int nc_paged_attn(const nc_tensor* q, const nc_paged_cache* cache, co
                  "paged_attn: q and out are not %d aligned rows of %d values", b->max_tokens, cols);
     NC_CHECK_ARG((q->dtype == NC_F16 || q->dtype == NC_Q8) && (out->dtype == NC_F16 || out->dtype == NC_Q8),
                  "paged_attn: dtypes %d, %d (F16 or Q8)", q->dtype, out->dtype);
-    const size_t need = attn_ws_bytes(attn_plan(a, cache->d_head), cache->d_head);
-    NC_CHECK_ARG(need <= workspace_bytes && (!need || (workspace && aligned16(workspace))),
-                 "paged_attn: workspace of %zu bytes (needs %zu, 16-byte aligned)", workspace_bytes, need);
-    if (b->max_tokens == 0 || b->max_new == 0 || b->max_kv == 0) return NC_OK;
+    NC_CHECK_ARG(!rows_overlap(q, out, b->max_tokens) || same_rows(q, out), "paged_attn: out lies over q but is not q");
     a.q = (const uint8_t*)q->data;
     a.q_pitch = q->pitch;
     a.q_dtype = q->dtype;
     a.out = (uint8_t*)out->data;
     a.out_pitch = out->pitch;
     a.out_dtype = out->dtype;
-    a.ws = (float*)workspace;
+    AttnPlan p = attn_plan(a, cache->d_head);
+    const size_t need = attn_ws_bytes(p, cache->d_head);
+    NC_CHECK_ARG(need <= workspace_bytes && (!need || (workspace && aligned16(workspace))),
+                 "paged_attn: workspace of %zu bytes (needs %zu, 16-byte aligned)", workspace_bytes, need);
+    if (b->max_tokens == 0 || b->max_new == 0 || b->max_kv == 0) return NC_OK;
+    p.rows.ws = (float*)workspace;
+    p.few.ws = (float*)((uint8_t*)workspace + rows_ws_bytes(p, cache->d_head));
     hipStream_t st = stream_of(stream);
-    const AttnPlan p = attn_plan(a, cache->d_head);
     if (cache->dtype == NC_Q8) return cache->d_head == 64 ? attn_launch<64, Q8>(p, st) : attn_launch<128, Q8>(p, st);
     return cache->d_head == 64 ? attn_launch<64, F16>(p, st) : attn_launch<128, F16>(p, st);
 }

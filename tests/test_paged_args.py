@@ -191,3 +191,44 @@ def test_nothing_to_do_is_no_error(nc):
     assert L.nc_paged_attn(C.byref(q), C.byref(cache), C.byref(batch), C.byref(q), 4, 0, 0, None, 0, None) == 0
     assert L.nc_paged_append(C.byref(q), C.byref(kv), C.byref(kv), C.byref(q), C.byref(cache), C.byref(batch), None, 0, 0,
                              None) == 0
+
+
+def test_results_over_inputs(nc):
+    L = nc.lib()
+    cache, batch, _ = structs(nc)
+    at = 1 << 20
+    row = lambda dtype, cols, data=at, pitch=0: nc.Tensor(data, None, dtype, 4, cols, pitch or  # noqa: E731
+                                                          cols * (2 if dtype == nc.F16 else 4))
+    q = row(nc.F16, 256)
+    q8 = nc.Tensor(at, None, nc.Q8, 4, 256, 272)
+    for out in (row(nc.F16, 256, at + 512), row(nc.F16, 256, at - 16), row(nc.F16, 256, at, 528), q8):
+        refused(nc, L.nc_paged_attn(C.byref(q), C.byref(cache), C.byref(batch), C.byref(out), 4, 0, 0, None, 0, None),
+                "lies over q")
+    lora = nc.Lora(a=16, b=16, scale=16, n_adapters=3, rank=16, k=64, n=64)
+    x, y = row(nc.F16, 64), row(nc.F32, 64, at << 1)
+
+    def add(out, x=x, y=y):
+        return L.nc_lora_add(C.byref(x), C.byref(y), C.byref(lora), 16, 16, 2, 2, C.byref(out), None)
+
+    refused(nc, add(x), "over x")
+    refused(nc, add(row(nc.F16, 64, at + 256)), "over x")
+    refused(nc, add(row(nc.F32, 64, at - 512)), "over x")
+    refused(nc, add(row(nc.F16, 64, at << 1)), "over base")
+    refused(nc, add(row(nc.F32, 64, (at << 1) + 256)), "over base")
+    refused(nc, add(row(nc.F32, 64, at << 1, 272)), "over base")
+
+
+def test_workspace_follows_the_rows_that_can_use_it(nc):
+    """One long chunk, or a few rows of it: not the rows of the chunk times the parts of a few."""
+    L, size = nc.lib(), C.c_size_t()
+    cache, batch, _ = structs(nc)
+    cache.n_kv_heads, cache.d_head, cache.n_pages = 8, 128, 1 << 16
+    batch.n_req, batch.max_tokens, batch.max_new, batch.max_kv, batch.max_pages = 1, 8192, 8192, 8192, 512
+    nc.check(L.nc_paged_attn_workspace(C.byref(cache), C.byref(batch), 64, 0, 0, C.byref(size)))
+    assert size.value < 64 << 20
+    for n_req in (1, 64, 4096):
+        for kv in (8192, 1 << 24):
+            batch.n_req, batch.max_tokens, batch.max_new, batch.max_kv, batch.max_pages = n_req, n_req, 1, kv, kv // 16
+            if n_req * batch.max_pages < 1 << 31:
+                nc.check(L.nc_paged_attn_workspace(C.byref(cache), C.byref(batch), 64, 0, 0, C.byref(size)))
+                assert size.value <= 1 << 30

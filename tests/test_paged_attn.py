@@ -344,3 +344,26 @@ def test_many_requests(gpu, n_req):
         attend(s, cache, q, out, hq)
         sync()
         check(s, cache, q, out, hq)
+
+
+@pytest.mark.parametrize("rows,ckind", [("f16", "f16"), ("q8", "q8"), ("f16", "q8")])
+def test_q_in_place(gpu, rows, ckind):
+    """out may be q: every kind of tile, joined parts among them, reads a row's head before it writes it."""
+    s, cache, q = make([1, 0, 3, 40, 150], [5000, 4, 700, 64, 300], 32, 64, 4, 2, rows, ckind, seed=18, pad=2)
+    out = Rows(rows, s.max_tokens, 256)
+    attend(s, cache, q, out, 4)
+    attend(s, cache, q, q, 4)
+    sync()
+    assert torch.equal(q.buf[:s.tokens], out.buf[:s.tokens])
+
+
+@pytest.mark.parametrize("new,past", [([1, 1, 1], [100, 3000, 0]), ([1, 20, 0, 130], [900, 5, 70, 2000])])
+@pytest.mark.parametrize("d,ckind", [(64, "q8"), (128, "f16")])
+def test_looser_bounds(gpu, new, past, d, ckind):
+    """Bounds far above the lengths: parts and tiles that hold nothing, other shapes of the launch."""
+    for max_new, max_kv in ((200, 2200), (1000, 70000), (200, 1 << 20)):
+        s, cache, q = make(new, past, 32, d, 4, 2, "f16", ckind, seed=19, max_new=max_new, max_kv=max(max_kv, 3001))
+        out = Rows("f16", s.max_tokens, 4 * d)
+        attend(s, cache, q, out, 4)
+        sync()
+        check(s, cache, q, out, 4)
