@@ -17,11 +17,15 @@
 // between lanes.
 //
 // Roundings: scores, statistics and sums are fp32.  What the matrix cores take
-// is fp16: in sixteen-row tiles each factor with more bits as two halves that
-// sum to it, so nothing is lost there; in 128-row tiles probabilities, Q8
-// values and Q8 q rows rounded once (2^-11 each; an fp16 result rounds as
-// much), for there the matrix cores are a bound and a second half would double
-// their work.  Probabilities are scaled by 2^14, so that what falls under
+// is fp16: each factor with more bits as two halves that sum to it, so that
+// nothing is lost there (of the products of two low halves nothing is left);
+// but over an fp16 cache the 128-row tiles round probabilities and Q8 q rows
+// once (2^-11 each, as an fp16 result), since second halves of those would take
+// half as many matrix instructions again.  Over a Q8 cache these tiles do keep
+// them, for 131 instead of 100 us (4 chunks of 500 rows over 2000 positions,
+// 32 heads over 4 of 64): its result rows may be Q8, whose codes turn with an
+// error far below their step (relative error of such rows 2.6e-3 with one
+// rounding each, 2.2e-4 without).  Probabilities are scaled by 2^14, so that what falls under
 // fp16's smallest number is below 2^-38 of the maximum's weight.
 #include "nc_act.h"
 #include "nc_paged.h"
@@ -578,7 +582,10 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 3) void k_paged_attn16(AttnArgs 
 // Sixteen-byte pieces of both are exchanged within rows by a function of the
 // row, so that sixteen neighbouring lanes' reads spread over all banks.
 //
-// Q8 values and q rows enter as their fp16 products, rounded once (2^-11).
+// Over an fp16 cache a step computes the next one's scores between its
+// exponentials; over a Q8 cache, with second halves to keep, the registers do
+// not hold two steps' scores (it took 136 us to 131, and 404 to 351 for heads
+// of 128), and the exponentials stand between the products with V instead.
 //
 // Bound by the instructions issued around the matrix ones (a wavefront issues
 // one every 7 cycles, four on a SIMD one every 3; per step of 64 positions
@@ -679,27 +686,31 @@ struct KvRows {
         }
     }
 
-    __device__ __forceinline__ void store_k(uint8_t* kb) const
+    // lo: where the second halves lie, from the first ones on
+    __device__ __forceinline__ void store_k(uint8_t* kb, int lo) const
     {
         const int tid = threadIdx.x;
 #pragma unroll
         for (int i = 0; i < kNk; i++) {
             const int at = i * 256 + tid, key = at / (D / 8), c = at % (D / 8);
-            u32x4 w;
-            if constexpr (CDT == F16) w = k[i];
-            else w = __builtin_bit_cast(u32x4, dequant8(kc[i], kd[i]).hi);
-            *reinterpret_cast<u32x4*>(kb + k_place<D>(key, c)) = w;
+            if constexpr (CDT == F16) {
+                *reinterpret_cast<u32x4*>(kb + k_place<D>(key, c)) = k[i];
+            } else {
+                const HalfPair8 w = dequant8(kc[i], kd[i]);
+                *reinterpret_cast<half8*>(kb + k_place<D>(key, c)) = w.hi;
+                *reinterpret_cast<half8*>(kb + lo + k_place<D>(key, c)) = w.lo;
+            }
         }
     }
 
     // Positions that are not to be seen are cleared; *not_finite = 1 where
     // rows that see a value that is no number and rows that do not may meet.
     // `part`: some of the tile's rows do not see all of the step at pos.
-    __device__ __forceinline__ void store_v(uint8_t* vb, const AttnArgs& a, const Seen& see, bool part, int pos,
+    __device__ __forceinline__ void store_v(uint8_t* vb, int lo, const AttnArgs& a, const Seen& see, bool part, int pos,
                                             bool page, int* not_finite) const
     {
         const int tid = threadIdx.x;
-        uint2 w[4];
+        uint2 w[4], wl[CDT == Q8 ? 4 : 1];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             if constexpr (CDT == F16) {
@@ -708,8 +719,10 @@ struct KvRows {
                 const _Float16 d = __builtin_bit_cast(_Float16, vd[j]);
                 half2v x[2];
                 codes4(vc[j], x);
-                w[j] = make_uint2(__builtin_bit_cast(uint32_t, x[0] * half2v{d, d}),
-                                  __builtin_bit_cast(uint32_t, x[1] * half2v{d, d}));
+                const half2v d2 = {d, d}, h0 = x[0] * d2, h1 = x[1] * d2;
+                w[j] = make_uint2(__builtin_bit_cast(uint32_t, h0), __builtin_bit_cast(uint32_t, h1));
+                wl[j] = make_uint2(__builtin_bit_cast(uint32_t, __builtin_elementwise_fma(x[0], d2, -h0)),
+                                   __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(x[1], d2, -h1)));
             }
         }
         if (part) {
@@ -720,35 +733,46 @@ struct KvRows {
                 const uint32_t keep = page & (p < see.hi) & ((p >= see.lo) | (p < a.sink)) ? ~0u : 0u;
                 w[j].x &= keep;
                 w[j].y &= keep;
+                if constexpr (CDT == Q8) {
+                    wl[j].x &= keep;
+                    wl[j].y &= keep;
+                }
                 odd |= pair_not_finite(w[j].x) | pair_not_finite(w[j].y);
             }
             if (odd) *not_finite = 1;
         }
         const int dg = tid % kDg, quad = tid / kDg;  // four positions: the piece and its half
         const int c = (quad >> 2) * 2 + (quad & 1), half = (quad >> 1) & 1;
+        auto put = [&](const uint2 (&w)[4], uint8_t* to) {
 #pragma unroll
-        for (int e = 0; e < kE; e++) {
-            const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
-            const uint32_t x0 = e < 2 ? w[0].x : w[0].y, x1 = e < 2 ? w[1].x : w[1].y;
-            const uint32_t x2 = e < 2 ? w[2].x : w[2].y, x3 = e < 2 ? w[3].x : w[3].y;
-            *reinterpret_cast<uint2*>(vb + v_place<D>(dg * kE + e, c) + half * 8) =
-                make_uint2(__builtin_amdgcn_perm(x1, x0, sel), __builtin_amdgcn_perm(x3, x2, sel));
-        }
+            for (int e = 0; e < kE; e++) {
+                const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
+                const uint32_t x0 = e < 2 ? w[0].x : w[0].y, x1 = e < 2 ? w[1].x : w[1].y;
+                const uint32_t x2 = e < 2 ? w[2].x : w[2].y, x3 = e < 2 ? w[3].x : w[3].y;
+                *reinterpret_cast<uint2*>(to + v_place<D>(dg * kE + e, c) + half * 8) =
+                    make_uint2(__builtin_amdgcn_perm(x1, x0, sel), __builtin_amdgcn_perm(x3, x2, sel));
+            }
+        };
+        put(w, vb);
+        if constexpr (CDT == Q8) put(wl, vb + lo);
     }
 };
 
-template <int D>
+template <int D, int CDT>
 struct SharedRows {
-    uint8_t kv[4][rows_step(D) * D * 2];  // two K and two V buffers
+    uint8_t kv[CDT == Q8 ? 8 : 4][rows_step(D) * D * 2];  // two K and two V buffers, then those of second halves
     Places places;
     int odd;
 };
 
 // Workgroup b of the 128-row tiles.
 template <int D, int CDT, int QDT>
-__device__ __forceinline__ void attn_rows(const AttnArgs& a, int b, SharedRows<D>& sh)
+__device__ __forceinline__ void attn_rows(const AttnArgs& a, int b, SharedRows<D, CDT>& sh)
 {
     constexpr int kS = rows_step(D), kG = kS / 16, kU = kS / 32, kKs = D / 16, kDt = D / 32, kBytes = kS * D * 2;
+    constexpr bool kNext = CDT == F16;      // scores a step ahead
+    constexpr int kAheadS = kNext ? 2 : 1;  // steps from the one at work to that whose K is on its way
+    constexpr int kLo = 4 * kBytes;  // from a buffer to that of its second halves
     Places& places = sh.places;
     int& odd_sh = sh.odd;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -774,12 +798,17 @@ __device__ __forceinline__ void attn_rows(const AttnArgs& a, int b, SharedRows<D
     const int my = min(first + c, t.n_rows - 1);
     const int my_tok = my / a.group, my_pos = t.pos0 + my_tok, my_lo = a.window ? my_pos - a.window + 1 : 0;
     const int w_lo = min(first, t.n_rows - 1) / a.group, w_hi = min(first + 31, t.n_rows - 1) / a.group;
-    half8 q[kKs];
+    constexpr bool kTwoQ = CDT == Q8 && QDT == Q8;
+    half8 q[kKs], q_lo[kTwoQ ? kKs : 1];
     {
         const uint8_t* row = a.q + (size_t)(t.first_row + my_tok) * a.q_pitch;
         const int col = (head * a.group + my % a.group) * D;
 #pragma unroll
-        for (int ks = 0; ks < kKs; ks++) q[ks] = q_values<QDT>(row, col + ks * 16 + h * 8, a.hq * D).hi;
+        for (int ks = 0; ks < kKs; ks++) {
+            const HalfPair8 w = q_values<QDT>(row, col + ks * 16 + h * 8, a.hq * D);
+            q[ks] = w.hi;
+            if constexpr (kTwoQ) q_lo[ks] = w.lo;
+        }
     }
     if (tid == 0) odd_sh = 0;
     __syncthreads();
@@ -816,18 +845,25 @@ __device__ __forceinline__ void attn_rows(const AttnArgs& a, int b, SharedRows<D
             __syncthreads();
             const bool some_none = places.some_none != 0;
 
-            // Step i computes the scores of step i + 1 between its exponentials, then
-            // multiplies those with its V; K of step i + 2 and V of step i + 1 are on
-            // their way from memory.
+            // Step i multiplies its probabilities with its V, and computes the
+            // scores of step i + kAheadS - 1; K of step i + kAheadS and V of step
+            // i + 1 are on their way from memory.
             auto clamped = [&](int i) { return min(i, vn - 1); };
             auto pos_of = [&](int i) { return steps.at(vt + clamped(i)) * kS; };
-            half8 kf[kKs][kU];
-            auto read_k = [&](const uint8_t* kb) {
-#pragma unroll
-                for (int ks = 0; ks < kKs; ks++)
-#pragma unroll
-                    for (int u = 0; u < kU; u++)
-                        kf[ks][u] = *reinterpret_cast<const half8*>(kb + k_place<D>(u * 32 + c, ks * 2 + h));
+            // K's operands, and those of second halves, some of them ahead
+            constexpr int kN = kKs * kU, kAheadK = CDT == Q8 ? 2 : kN;
+            half8 kf[kAheadK], kl[CDT == Q8 ? kAheadK : 1];
+            auto read_k = [&](const uint8_t* kb, int n) {
+                const int at = k_place<D>(n % kU * 32 + c, n / kU * 2 + h);
+                kf[n % kAheadK] = *reinterpret_cast<const half8*>(kb + at);
+                if constexpr (CDT == Q8) kl[n % kAheadK] = *reinterpret_cast<const half8*>(kb + kLo + at);
+            };
+            // the n-th product of K and q, second halves too
+            auto score = [&](const uint8_t* kb, int n, f32x16& s) {
+                s = mfma32(kf[n % kAheadK], q[n / kU], s);
+                if constexpr (kTwoQ) s = mfma32(kf[n % kAheadK], q_lo[n / kU], s);
+                if constexpr (CDT == Q8) s = mfma32(kl[n % kAheadK], q[n / kU], s);
+                if (n + kAheadK < kN) read_k(kb, n + kAheadK);
             };
             // whether all rows from token lo to hi see the whole step at pos
             auto all_see = [&](int pos, int lo, int hi) {
@@ -845,44 +881,56 @@ __device__ __forceinline__ void attn_rows(const AttnArgs& a, int b, SharedRows<D
             auto store_v = [&](const KvRows<D, CDT>& from, uint8_t* vb, int i) {
                 const int pos = pos_of(i), e = clamped(i) * kG + KvRows<D, CDT>::v_sixteen(wave);
                 const bool page = !some_none || !((places.none[e >> 5] >> (e & 31)) & 1);
-                from.store_v(vb, a, see, !all_see(pos, t.tok_lo, t.tok_hi), pos, page, &odd_sh);
+                from.store_v(vb, kLo, a, see, !all_see(pos, t.tok_lo, t.tok_hi), pos, page, &odd_sh);
             };
             KvRows<D, CDT> kv;
-            f32x16 s[kU], t_s[kU];
-            {
+            f32x16 s[kU], t_s[kNext ? kU : 1];
+            places_of(0, 0);
+            kv.load_k(a, k_at0, k_at1, wave);
+            kv.load_v(a, v_at, wave);
+            if constexpr (kNext) {
                 KvRows<D, CDT> w;
-                places_of(0, 0);
-                kv.load_k(a, k_at0, k_at1, wave);
-                kv.load_v(a, v_at, wave);
                 places_of(1, 1);
                 w.load_k(a, k_at0, k_at1, wave);
                 places_of(2, 1);
-                kv.store_k(k_sh[0]);
+                kv.store_k(k_sh[0], kLo);
                 store_v(kv, v_sh[0], 0);
-                w.store_k(k_sh[1]);
+                w.store_k(k_sh[1], kLo);
+            } else {
+                places_of(1, 1);
+                kv.store_k(k_sh[0], kLo);
+                store_v(kv, v_sh[0], 0);
             }
             __syncthreads();
-            read_k(k_sh[0]);
+            if constexpr (kNext) {
 #pragma unroll
-            for (int u = 0; u < kU; u++) s[u] = t_s[u] = f32x16{};
+                for (int n = 0; n < kAheadK; n++) read_k(k_sh[0], n);
 #pragma unroll
-            for (int ks = 0; ks < kKs; ks++)
+                for (int u = 0; u < kU; u++) s[u] = t_s[u] = f32x16{};
 #pragma unroll
-                for (int u = 0; u < kU; u++) s[u] = mfma32(kf[ks][u], q[ks], s[u]);
-            __syncthreads();
-            auto step = [&](f32x16 (&s)[kU], f32x16 (&s_next)[kU], int i0, int buf) {
-                if (i0 + 2 < vn) kv.load_k(a, k_at0, k_at1, wave);
+                for (int n = 0; n < kN; n++) score(k_sh[0], n, s[n % kU]);
+                __syncthreads();
+            }
+            auto step = [&](f32x16 (&s)[kU], auto& s_next, int i0, int buf) {
+                if (i0 + kAheadS < vn) kv.load_k(a, k_at0, k_at1, wave);
                 if (i0 + 1 < vn) kv.load_v(a, v_at, wave);
-                places_of(i0 + 3, i0 + 2);
+                places_of(i0 + kAheadS + 1, i0 + 2);
                 const int pos = pos_of(i0);
                 // unless the wavefront sees none of the step's positions
                 if (mine && pos <= t.pos0 + w_hi) {
                     const uint8_t* vb = v_sh[buf];
-                    auto read_v = [&](int i) {  // operand i: values 32 (i % kDt) of sixteen i / kDt
-                        return *reinterpret_cast<const half8*>(vb + v_place<D>(i % kDt * 32 + c, i / kDt * 2 + h));
+                    auto read_v = [&](int i, int lo) {  // operand i: values 32 (i % kDt) of sixteen i / kDt
+                        return *reinterpret_cast<const half8*>(vb + lo + v_place<D>(i % kDt * 32 + c, i / kDt * 2 + h));
                     };
-                    constexpr int kNv = 2 * kU * kDt, kAhead = D == 128 ? 4 : 8;
-                    read_k(k_sh[buf ^ 1]);
+                    constexpr int kNv = 2 * kU * kDt, kAhead = D == 128 || CDT == Q8 ? 4 : 8;
+#pragma unroll
+                    for (int n = 0; n < kAheadK; n++) read_k(k_sh[buf ^ (kNext ? 1 : 0)], n);
+                    if constexpr (!kNext) {
+#pragma unroll
+                        for (int u = 0; u < kU; u++) s[u] = f32x16{};
+#pragma unroll
+                        for (int n = 0; n < kN; n++) score(k_sh[buf], n, s[n % kU]);
+                    }
                     if (!all_see(pos, w_lo, w_hi)) {
                         // against the lane's first position: its others lie at constants
                         const int at0 = pos + 4 * h, hi = my_pos - at0, lo = my_lo - at0, sk = a.sink - at0;
@@ -913,38 +961,74 @@ __device__ __forceinline__ void attn_rows(const AttnArgs& a, int b, SharedRows<D
                     // Each matrix instruction of the next step's scores between some
                     // of this step's exponentials: in a run of their own each kind
                     // leaves the other's unit idle, in step with the other wavefronts.
-                    half8 p[2 * kU], vf[kAhead];
+                    half8 p[2 * kU], p_lo[CDT == Q8 ? 2 * kU : 1], vf[kAhead], vl[CDT == Q8 ? kAhead : 1];
 #pragma unroll
-                    for (int i = 0; i < kAhead; i++) vf[i] = read_v(i);
-                    constexpr int kN = kKs * kU, kEach = 16 * kU / kN;
-#pragma unroll
-                    for (int u = 0; u < kU; u++) s_next[u] = f32x16{};
-#pragma unroll
-                    for (int n = 0; n < kN; n++) {
-                        s_next[n % kU] = mfma32(kf[n / kU][n % kU], q[n / kU], s_next[n % kU]);
-#pragma unroll
-                        for (int i = n * kEach; i < (n + 1) * kEach; i++)
-                            p[i >> 3][i & 7] =
-                                (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 4][i & 15], a.scale, -base));
-                        __builtin_amdgcn_sched_barrier(0);
+                    for (int i = 0; i < kAhead; i++) {
+                        vf[i] = read_v(i, 0);
+                        if constexpr (CDT == Q8) vl[i] = read_v(i, kLo);
                     }
-#pragma unroll
-                    for (int i = 0; i < kNv; i++) {
+                    auto weigh = [&](int i) {  // probability i
+                        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 4][i & 15], a.scale, -base));
+                        p[i >> 3][i & 7] = (_Float16)e;
+                        if constexpr (CDT == Q8) {
+                            sum += e;
+                            p_lo[i >> 3][i & 7] = (_Float16)(e - (float)p[i >> 3][i & 7]);
+                        }
+                    };
+                    auto add_v = [&](int i) {  // operand i, its probabilities among p[i / kDt]
                         const half8 f = vf[i % kAhead];
-                        if (i + kAhead < kNv) vf[i % kAhead] = read_v(i + kAhead);
+                        if (i + kAhead < kNv) vf[i % kAhead] = read_v(i + kAhead, 0);
                         o[i % kDt] = mfma32(f, p[i / kDt], o[i % kDt]);
-                        if (i % kDt == kDt - 1) sum = sum8(p[i / kDt], sum);
-                        __builtin_amdgcn_sched_barrier(0);
+                        if constexpr (CDT == Q8) {
+                            const half8 f_lo = vl[i % kAhead];
+                            if (i + kAhead < kNv) vl[i % kAhead] = read_v(i + kAhead, kLo);
+                            o[i % kDt] = mfma32(f, p_lo[i / kDt], o[i % kDt]);
+                            o[i % kDt] = mfma32(f_lo, p[i / kDt], o[i % kDt]);
+                        } else if (i % kDt == kDt - 1) {
+                            sum = sum8(p[i / kDt], sum);
+                        }
+                    };
+                    if constexpr (kNext) {
+                        constexpr int kEach = 16 * kU / kN;
+#pragma unroll
+                        for (int u = 0; u < kU; u++) s_next[u] = f32x16{};
+#pragma unroll
+                        for (int n = 0; n < kN; n++) {
+                            score(k_sh[buf ^ 1], n, s_next[n % kU]);
+#pragma unroll
+                            for (int i = n * kEach; i < (n + 1) * kEach; i++) weigh(i);
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+#pragma unroll
+                        for (int i = 0; i < kNv; i++) {
+                            add_v(i);
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                    } else {
+                        constexpr int kEach = 8 / kDt;
+#pragma unroll
+                        for (int i = 0; i < 8; i++) weigh(i);
+#pragma unroll
+                        for (int i = 0; i < kNv; i++) {
+                            add_v(i);
+#pragma unroll
+                            for (int j = 8 + i * kEach; j < 8 + (i + 1) * kEach; j++)
+                                if (j < 16 * kU) weigh(j);
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
                     }
                 }
                 // what these overwrite was last read before the last barrier
-                if (i0 + 2 < vn) kv.store_k(k_sh[buf]);
+                if (i0 + kAheadS < vn) kv.store_k(k_sh[buf ^ (kNext ? 0 : 1)], kLo);
                 if (i0 + 1 < vn) store_v(kv, v_sh[buf ^ 1], i0 + 1);
                 __syncthreads();
             };
             for (int i0 = 0; i0 < vn; i0 += 2) {
                 step(s, t_s, i0, 0);
-                if (i0 + 1 < vn) step(t_s, s, i0 + 1, 1);
+                if (i0 + 1 < vn) {
+                    if constexpr (kNext) step(t_s, s, i0 + 1, 1);
+                    else step(s, t_s, i0 + 1, 1);
+                }
             }
         }
         sum += __shfl_xor(sum, 32);
@@ -1016,7 +1100,7 @@ template <int D, int CDT, int QDT>
 __global__ __launch_bounds__(256, 2) void k_paged_mixed(MixedArgs a)
 {
     __shared__ union {
-        SharedRows<D> rows;
+        SharedRows<D, CDT> rows;
         Shared16<D> few;
     } sh;
     if ((int)blockIdx.x < a.row_blocks) attn_rows<D, CDT, QDT>(a.rows, blockIdx.x, sh.rows);

@@ -197,14 +197,17 @@ def visible(p, kv, window, sink):
     return seen & ((j > p - window) | (j < sink)) if window else seen
 
 
-def plain_attention(step, cache, q, hq, window=0, sink=0, hidden=None, eps_k=0.0, eps_v=0.0, eps_q=0.0):
+def plain_attention(step, cache, q, hq, window=0, sink=0, hidden=None):
     """64-bit results [tokens, hq * d] and, for each value, how far the kernel's documented roundings can take it.
 
-    Errors, to first order: a probability's rounding to fp16 (HALF of itself), V's (eps_v), and of the scores those of
-    q and k (eps_q, eps_k of sum |q k| / sqrt d), which change a weight by their difference from the row's mean change;
-    fp32 sums and exp2 of a few hundred terms are held to 2^-16 of the terms' magnitudes."""
+    Over an fp16 cache, to first order: a probability's rounding to fp16 (HALF of itself) and, of Q8 q rows, that of the
+    scores (HALF of sum |q k| / sqrt d), which changes a weight by its difference from the row's mean change.  Over a Q8
+    cache nothing enters rounded.  fp32 sums and exp2 of a few hundred terms are held to 2^-16 of the terms' magnitudes,
+    scores to 2^-20."""
     n_pages, hkv, page, d = cache.shape
     group = hq // hkv
+    eps_p = HALF if cache.kind == "f16" else 0.0
+    eps_q = HALF if cache.kind == "f16" and q.kind == "q8" else 0.0
     qv = q.values().reshape(-1, hq, d)
     out = torch.zeros(step.tokens, hq, d, dtype=torch.float64)
     tol = torch.zeros_like(out)
@@ -226,8 +229,8 @@ def plain_attention(step, cache, q, hq, window=0, sink=0, hidden=None, eps_k=0.0
             w = torch.softmax(s, -1)
             out[first + i] = torch.einsum("hj,jhd->hd", w, vv)
             weight = torch.einsum("hj,jhd->hd", w, vv.abs())
-            ds = (mag * (eps_k + eps_q + 2.0 ** -20)).amax(-1, keepdim=True)
-            tol[first + i] = weight * (HALF + eps_v + 2 * ds + 2.0 ** -16) + TINY
+            ds = (mag * (eps_q + 2.0 ** -20)).amax(-1, keepdim=True)
+            tol[first + i] = weight * (eps_p + 2 * ds + 2.0 ** -16) + TINY
     return out.reshape(step.tokens, hq * d), tol.reshape(step.tokens, hq * d)
 
 

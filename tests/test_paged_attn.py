@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import paged_util as P
-from paged_util import HALF, Cache, Rows, Step, attend, plain_attention, rounded, sync, within, workspace
+from paged_util import Cache, Rows, Step, attend, plain_attention, rounded, sync, within, workspace
 
 pytestmark = pytest.mark.gpu
 
@@ -25,9 +25,7 @@ def make(new, past, page, d, hq, hkv, rows, ckind, seed=0, pad=0, fill=float("na
 
 
 def check(s, cache, q, out, hq, window=0, sink=0, hidden=None, what=""):
-    eps_k = eps_v = HALF if cache.kind == "q8" else 0.0
-    want, tol = plain_attention(s, cache, q, hq, window, sink, hidden, eps_k=eps_k, eps_v=eps_v,
-                                eps_q=HALF if q.kind == "q8" else 0.0)
+    want, tol = plain_attention(s, cache, q, hq, window, sink, hidden)
     got = out.values()[:s.tokens]
     assert torch.isfinite(got).all(), what
     within(got, want, rounded(out.kind, want, tol), what)

@@ -11,7 +11,7 @@ import pytest
 import torch
 
 import paged_util as P
-from paged_util import HALF, Cache, Rows, ints, plain_attention, rounded, sync, within, workspace
+from paged_util import Cache, Rows, ints, plain_attention, rounded, sync, within, workspace
 
 pytestmark = pytest.mark.gpu
 
@@ -136,8 +136,7 @@ def test_steps(gpu, kind, window, sink):
             for name, rows in (("k", turned), ("v", vv)):
                 want = Rows(kind, n, HKV * D, rows.values().float()).values()
                 assert torch.equal(cache.values(name, sv.past_slots(r)).reshape(n, -1), want), (step, r, name)
-        eps = HALF if kind == "q8" else 0.0
-        want, tol = plain_attention(sv, cache, qr, HQ, window, sink, eps_k=eps, eps_v=eps, eps_q=eps)
+        want, tol = plain_attention(sv, cache, qr, HQ, window, sink)
         within(att.values()[live], want, rounded(kind, want, tol), f"attention, step {step}")
         assert torch.isfinite(y.values()[live]).all()
         gpu.check(L.nc_paged_commit(sv.pool_ref, sv.ref, P.ptr(sv.finished), None), "commit")
