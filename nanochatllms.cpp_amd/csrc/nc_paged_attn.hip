@@ -22,8 +22,8 @@
 // but over an fp16 cache the 128-row tiles round probabilities and Q8 q rows
 // once (2^-11 each, as an fp16 result), since second halves of those would take
 // half as many matrix instructions again.  Over a Q8 cache these tiles do keep
-// them, for 131 instead of 100 us (4 chunks of 500 rows over 2000 positions,
-// 32 heads over 4 of 64): its result rows may be Q8, whose codes turn with an
+// them, for 131 instead of 100 us (4 chunks of 500 rows over up to 2000
+// positions, 32 heads over 4 of 64): its result rows may be Q8, whose codes turn with an
 // error far below their step (relative error of such rows 2.6e-3 with one
 // rounding each, 2.2e-4 without).  Probabilities are scaled by 2^14, so that what falls under
 // fp16's smallest number is below 2^-38 of the maximum's weight.
@@ -53,6 +53,7 @@ struct AttnArgs {
     float scale;   // log2(e) / sqrt(d)
     int few;        // requests of at most this many (token, head) rows take sixteen-row tiles
     int row_tiles;  // sixteen-row tiles of a request
+    long long tiles;  // tile numbers, kv heads counted: the workgroups of one part
     int splits;     // parts of a tile's positions at most
     int part;       // steps of a part
     size_t lines;   // rows of a part in the workspace: max_tokens * hq, or
@@ -214,9 +215,9 @@ __device__ __forceinline__ f32x4 mfma16(half8 a, half8 b, f32x4 c)
 // both enter as two fp16 halves (of the products of two low halves nothing is
 // left), so the sums are as good as fp32 ones.  These tiles wait for memory,
 // not for the matrix cores: one token each of 64 requests of up to 8000
-// positions, 32 heads over 8 kv heads of 128, fp16, 1.1 GB: 233 us, 4.7 TB/s
+// positions, 32 heads over 8 kv heads of 128, fp16, 1.1 GB: 204 us, 5.4 TB/s
 // (a large copy reaches 4.8); of 40 requests of up to 3900, 36 kv heads of
-// 64, Q8, 397 MB: 108 us, 3.7 TB/s (turning the codes to fp16 fills the issue
+// 64, Q8, 413 MB: 106 us, 3.9 TB/s (turning the codes to fp16 fills the issue
 // slots as well).  One request of 700 positions: 8 us, two launches and the
 // latency of page lookup, K, V and the join.
 
@@ -355,8 +356,11 @@ __device__ __forceinline__ void attn16(const AttnArgs& a, int b, Shared16<D>& sh
     int& odd_sh = sh.odd;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 15, g = lane >> 4;
-    const int part = b % a.splits;
-    b /= a.splits;
+    // the parts one after the other: with a tile's side by side, the last parts,
+    // which ragged lengths leave short or empty, fall on the same XCDs (64
+    // requests of up to 8000 positions in two parts each: 233 to 215 us)
+    const int part = b / (int)a.tiles;
+    b -= part * (int)a.tiles;
     const size_t lines0 = (size_t)b * 16;
     const int head = b % a.hkv;
     b /= a.hkv;
@@ -591,9 +595,9 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 3) void k_paged_attn16(AttnArgs 
 // one every 7 cycles, four on a SIMD one every 3; per step of 64 positions
 // and 32 rows 32 exponentials, as many conversions and 64 scalings and maxima
 // stand against 16 matrix instructions of 33 cycles): 4 chunks of 500 rows
-// over 2000 positions, 32 heads over 4 kv heads of 64, 26 GFLOP: 60 us, 430
-// TFLOP/s; two of 1000 rows under a window of 1024, 8 kv heads of 128, 36
-// GFLOP: 88 us, 410 TFLOP/s.  Sixteen-row tiles took 139 and 248.
+// over up to 2000 positions, 32 heads over 4 kv heads of 64, 22 GFLOP: 60 us,
+// 370 TFLOP/s; two of 1000 rows under a window of 1024, 8 kv heads of 128, 35
+// GFLOP: 87 us, 400 TFLOP/s.  Sixteen-row tiles took 139 and 248.
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
@@ -779,10 +783,9 @@ __device__ __forceinline__ void attn_rows(const AttnArgs& a, int b, SharedRows<D
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     uint8_t (*k_sh)[kBytes] = sh.kv, (*v_sh)[kBytes] = sh.kv + 2;
     const int c = lane & 31, h = lane >> 5;
-    const int head = b % a.hkv;
-    b /= a.hkv;
-    const int part = b % a.splits;
-    const int slot = b / a.splits;
+    const int part = b / (int)a.tiles;
+    b -= part * (int)a.tiles;
+    const int head = b % a.hkv, slot = b / a.hkv;
     const TileRequest at = tile_request(a.row_start, a.kv_len, a.n_req, slot, a.group, kRowsM, a.max_tokens);
     const int req = at.req, row0 = (slot - first_tile(at.start, req, a.group, kRowsM, a.max_tokens)) * kRowsM;
     Tile t;
@@ -1220,17 +1223,17 @@ static void shape16(AttnArgs& a, int d)
 {
     const long long rows = (long long)(a.max_new < a.max_tokens ? a.max_new : a.max_tokens) * a.group;
     a.row_tiles = (int)(((rows < a.few ? rows : a.few) + 15) / 16);
-    const long long tiles = (long long)a.n_req * a.row_tiles * a.hkv, most = most_steps(a, 16, 32);
+    const long long tiles = a.tiles = (long long)a.n_req * a.row_tiles * a.hkv, most = most_steps(a, 16, 32);
     const long long by_token = (long long)a.max_tokens * a.hq;
     a.by_tile = tiles * 16 < by_token;
     a.lines = (size_t)(a.by_tile ? tiles * 16 : by_token);
     long long want = tiles > 0 ? (1024 + tiles - 1) / tiles : 1;
     if (want > (most + 3) / 4) want = (most + 3) / 4;  // a step for each wavefront
-    // With workgroups enough, parts of 4096 positions even out ragged lengths
-    // (64 requests of up to 8000, 8 kv heads of 128, parts of 1024, 2048 and
-    // 4096: 264, 239 and 232 us; 40 of up to 3900, 36 kv heads, Q8: 124, 116
-    // and 105), within 1 GB of workspace.
-    long long by_len = (most + 127) / 128;
+    // With workgroups enough, parts of 1024 positions even out ragged lengths
+    // (64 requests of up to 8000, 8 kv heads of 128, parts of 512, 1024, 2048
+    // and 4096: 209, 204, 206 and 215 us; 40 of up to 3900, 36 kv heads, Q8:
+    // 111, 106, 108 and 113), within 1 GB of workspace.
+    long long by_len = (most + 31) / 32;
     const long long room = a.lines ? (1ll << 30) / ((long long)a.lines * (d + 2) * 4) : 1;
     if (by_len > room) by_len = room;
     if (want < by_len && tiles < 65536) want = by_len;
@@ -1242,10 +1245,18 @@ static void shape_rows(AttnArgs& a, int d)
 {
     const int S = rows_step(d);
     const long long tiles = ((long long)a.max_tokens * a.group / kRowsM + 1) * a.hkv, most = most_steps(a, kRowsM, S);
+    a.tiles = tile_slots(a.max_tokens, a.n_req, a.group, kRowsM) * a.hkv;
     a.by_tile = false;
     a.lines = (size_t)a.max_tokens * a.hq;
     long long want = (512 + tiles - 1) / tiles;
     if (want > (most + 3) / 4) want = (most + 3) / 4;
+    // Where all tiles run at once the longest sets the time: parts of 1024
+    // positions (520 tiles, 4 chunks over up to 2500 positions, heads of 128:
+    // 91 to 88 us, Q8 234 to 197; 256 tiles over 5000: 85 to 73).  Where they
+    // take turns, parts only add their sums' traffic (1850 tiles: 185 to 228).
+    // Under a window all are of a length.
+    const long long by_len = (most * S + 1023) / 1024;
+    if (!a.window && tiles < 768 && want < by_len) want = by_len;
     set_parts(a, most, want, 1);
 }
 
@@ -1314,24 +1325,22 @@ template <int D, int CDT, int QDT>
 static int attn_launch(const AttnPlan& p, hipStream_t st)
 {
     const AttnArgs &f = p.few, &r = p.rows;
-    const long long tiles = (long long)f.n_req * f.row_tiles * f.hkv;
-    const long long slots = tile_slots(r.max_tokens, r.n_req, r.group, kRowsM) * r.hkv;
-    NC_CHECK_ARG(tiles * f.splits <= 0xFFFFFF && (!p.some_rows || slots * 8 * r.splits <= 0xFFFFFF),
-                 "paged_attn: %lld tiles of %d parts are too many for one launch", tiles > slots ? tiles : slots,
-                 p.some_rows && r.splits > f.splits ? r.splits : f.splits);
+    NC_CHECK_ARG(f.tiles * f.splits <= 0xFFFFFF && (!p.some_rows || r.tiles * 8 * r.splits <= 0xFFFFFF),
+                 "paged_attn: %lld tiles of %d parts are too many for one launch", p.some_rows ? r.tiles : f.tiles,
+                 p.some_rows ? r.splits : f.splits);
     if (p.some_rows) {
-        MixedArgs m{r, f, (int)(slots * r.splits)};
-        const unsigned grid = (unsigned)(m.row_blocks + tiles * f.splits);
+        MixedArgs m{r, f, (int)(r.tiles * r.splits)};
+        const unsigned grid = (unsigned)(m.row_blocks + f.tiles * f.splits);
         hipLaunchKernelGGL((k_paged_mixed<D, CDT, QDT>), dim3(grid), dim3(256), 0, st, m);
         if (f.splits > 1 || r.splits > 1) {
-            m.row_blocks = r.splits > 1 ? (int)(slots * (kRowsM / 16)) : 0;
-            const unsigned blocks = (unsigned)(m.row_blocks + (f.splits > 1 ? tiles : 0));
+            m.row_blocks = r.splits > 1 ? (int)(r.tiles * (kRowsM / 16)) : 0;
+            const unsigned blocks = (unsigned)(m.row_blocks + (f.splits > 1 ? f.tiles : 0));
             hipLaunchKernelGGL((k_paged_join_mixed<D>), dim3(blocks), dim3(16 * D / 8), 0, st, m);
         }
         return launch_status("k_paged_mixed");
     }
-    hipLaunchKernelGGL((k_paged_attn16<D, CDT, QDT>), dim3((unsigned)(tiles * f.splits)), dim3(256), 0, st, f);
-    if (f.splits > 1) hipLaunchKernelGGL((k_paged_join<D>), dim3((unsigned)tiles), dim3(16 * D / 8), 0, st, f);
+    hipLaunchKernelGGL((k_paged_attn16<D, CDT, QDT>), dim3((unsigned)(f.tiles * f.splits)), dim3(256), 0, st, f);
+    if (f.splits > 1) hipLaunchKernelGGL((k_paged_join<D>), dim3((unsigned)f.tiles), dim3(16 * D / 8), 0, st, f);
     return launch_status("k_paged_attn16");
 }
 
