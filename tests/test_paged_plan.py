@@ -142,6 +142,31 @@ def test_commit_takes_and_returns_pages(gpu):
     assert s.free_pages.tolist()[:len(free)] == free
 
 
+@pytest.mark.parametrize("n_req", [63, 1025, 4096])
+@pytest.mark.parametrize("share", [0.02, 0.5, 1.0])
+def test_commit_many_requests(gpu, n_req, share):
+    """Flags in more wavefronts and lots than one, pages in more than one load of a wavefront's."""
+    g = gen(n_req)
+    past = torch.randint(0, 60, (n_req,), generator=g).tolist()
+    past[n_req // 2] = 1500
+    s = Step([i % 3 for i in range(n_req)], past, 16, g)
+    plan(gpu, s)
+    done = (torch.rand(n_req, generator=g) < share).int().tolist()
+    done[n_req // 2] = -1
+    commit(gpu, s, ints(done))
+    sync()
+    free, table = list(s.want_free), [list(t) for t in s.want_table]
+    for r in range(n_req):
+        if done[r]:
+            n = P.up(s.new[r] + s.past[r], 16)
+            free += table[r][:n]
+            table[r][:n] = [-1] * n
+    assert s.state.tolist()[:3] == [len(free), len(free), 0]
+    assert s.free_pages.tolist()[:len(free)] == free
+    assert s.table.tolist() == table
+    assert s.seq_len.tolist() == [0 if f else n + p for f, n, p in zip(done, s.new, past)]
+
+
 def test_commit_passes_over_entries_that_are_no_page(gpu):
     s = Step([1], [79], 16, gen(7))
     plan(gpu, s)
