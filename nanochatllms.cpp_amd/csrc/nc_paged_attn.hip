@@ -55,7 +55,9 @@ struct AttnArgs {
     int row_tiles;  // sixteen-row tiles of a request
     long long tiles;  // tile numbers, kv heads counted: the workgroups of one part
     int splits;     // parts of a tile's positions at most
-    int part;       // steps of a part
+    int fill;       // parts of a tile that the chip has room for
+    float fill_inv; // 1 / fill
+    int longest;    // steps of a part at most, while `splits` of them hold all
     size_t lines;   // rows of a part in the workspace: max_tokens * hq, or
     bool by_tile;   // sixteen for each (sixteen-row tile, kv head), where those are fewer
     float* ws;      // [splits][lines][d] sums, then as many (maximum, sum) pairs
@@ -84,6 +86,30 @@ struct Steps {
     }
     __device__ __forceinline__ int at(int v) const { return v < sinks ? v : first + v - sinks; }
 };
+
+// Steps of a part, a multiple of UNIT, of a tile of `count` (at least 1): as
+// many parts as the chip has room for, though of no less than four steps, and
+// where those are long, parts of `longest` with a shorter last one (which
+// evens out better than parts alike).  By the steps that there are, not by the
+// bound that sizes the launch: with a bound 64 times the lengths that left one
+// part to each (64 requests of up to 2000: 130 us for 65).
+template <int UNIT>
+__device__ __forceinline__ int steps_of_part(const AttnArgs& a, int count)
+{
+    int each = count;
+    if (a.fill > 1) {
+        // ceil(count / fill) without a division, which cost the join 0.3 us
+        each = (int)((float)count * a.fill_inv);
+        each += each * a.fill < count;
+        each += each * a.fill < count;
+        each = max(each, 4);
+    }
+    if (each > a.longest) {
+        each = a.longest;
+        if ((long long)each * a.splits < count) each = (count + a.splits - 1) / a.splits;
+    }
+    return (each + UNIT - 1) / UNIT * UNIT;
+}
 
 // Rows [row0, row0 + M) of the request's (token, head) rows.
 struct Tile {
@@ -370,10 +396,9 @@ __device__ __forceinline__ void attn16(const AttnArgs& a, int b, Shared16<D>& sh
         t.n_rows > a.few)
         return;
     const Steps<32> steps(t.lo, t.hi, a.sink);
-    const int v0 = part * a.part;
-    if (v0 >= steps.count) return;
-    const int v1 = part == a.splits - 1 ? steps.count : min(v0 + a.part, steps.count);
-    const int parts = min((steps.count + a.part - 1) / a.part, a.splits);
+    const int each = steps_of_part<4>(a, steps.count), v0 = part * each, v1 = min(v0 + each, steps.count);
+    const bool parted = each < steps.count;
+    if (v0 >= v1) return;
 
     // this lane's row: q operand and position
     const int my = min(t.row0 + c, t.n_rows - 1);
@@ -543,7 +568,7 @@ __device__ __forceinline__ void attn16(const AttnArgs& a, int b, Shared16<D>& sh
 #pragma unroll
                 for (int i = 0; i < 8; i++) r[i] += f * o_sh[w][rr][c8 * 8 + i];
             }
-            if (parts == 1) {
+            if (!parted) {
                 const float inv = total != 0.0f ? 1.0f / total : 0.0f;
 #pragma unroll
                 for (int i = 0; i < 8; i++) r[i] *= inv;
@@ -791,10 +816,9 @@ __device__ __forceinline__ void attn_rows(const AttnArgs& a, int b, SharedRows<D
     Tile t;
     if (row0 < 0 || !tile_of<kRowsM>(a, at.start, at.end, at.of, row0, t) || t.n_rows <= a.few) return;
     const Steps<kS> steps(t.lo, t.hi, a.sink);
-    const int v0 = part * a.part;
-    if (v0 >= steps.count) return;
-    const int v1 = part == a.splits - 1 ? steps.count : min(v0 + a.part, steps.count);
-    const int parts = min((steps.count + a.part - 1) / a.part, a.splits);
+    const int each = steps_of_part<1>(a, steps.count), v0 = part * each, v1 = min(v0 + each, steps.count);
+    const bool parted = each < steps.count;
+    if (v0 >= v1) return;
 
     const int first = row0 + wave * 32;  // the wavefront's rows
     const bool mine = first < t.n_rows;
@@ -1044,7 +1068,7 @@ __device__ __forceinline__ void attn_rows(const AttnArgs& a, int b, SharedRows<D
 
             // lane (c, h): row c, values 32 dt + 8 j + 4 h + i
             const int tok = t.first_row + my_tok, qh = head * a.group + my % a.group;
-            if (parts > 1) {
+            if (parted) {
                 const size_t at = part * a.lines + (size_t)tok * a.hq + qh;
 #pragma unroll
                 for (int dt = 0; dt < kDt; dt++)
@@ -1139,10 +1163,10 @@ __device__ __forceinline__ void join_parts(const AttnArgs& a, int b)
         (M == 16 ? t.n_rows > a.few : t.n_rows <= a.few))
         return;
     const Steps<S> steps(t.lo, t.hi, a.sink);
-    const int parts = min((steps.count + a.part - 1) / a.part, a.splits);
+    const int each = steps_of_part<M == 16 ? 4 : 1>(a, steps.count);
     const int rr = threadIdx.x / (D / 8), c8 = threadIdx.x % (D / 8);
     const int row = t.row0 + sub * 16 + rr;
-    if (parts <= 1 || row >= t.n_rows) return;
+    if (each >= steps.count || row >= t.n_rows) return;
     const int tok = t.first_row + row / a.group, qh = head * a.group + row % a.group;
     const size_t line = M == 16 && a.by_tile ? lines0 + rr : (size_t)tok * a.hq + qh;
     const float2* ml = reinterpret_cast<const float2*>(a.ws + a.splits * a.lines * D) + line;
@@ -1151,12 +1175,12 @@ __device__ __forceinline__ void join_parts(const AttnArgs& a, int b)
     // several parts' loads in flight: one after the other, a part took the
     // memory's latency
     constexpr int kAhead = 8;
-    for (int s0 = 0; s0 < parts; s0 += kAhead) {
+    for (int s0 = 0; s0 * each < steps.count; s0 += kAhead) {
         float2 e[kAhead];
         float4 u[kAhead][2];
 #pragma unroll
         for (int i = 0; i < kAhead; i++) {
-            const int s = min(s0 + i, parts - 1);
+            const int s = (s0 + i) * each < steps.count ? s0 + i : s0;
             e[i] = ml[s * a.lines];
             u[i][0] = *reinterpret_cast<const float4*>(sums + s * a.lines * D);
             u[i][1] = *reinterpret_cast<const float4*>(sums + s * a.lines * D + 4);
@@ -1171,7 +1195,7 @@ __device__ __forceinline__ void join_parts(const AttnArgs& a, int b)
         for (int j = 0; j < 8; j++) r[j] *= keep;
 #pragma unroll
         for (int i = 0; i < kAhead; i++) {
-            if (s0 + i >= parts || e[i].x == -__builtin_inff()) continue;
+            if ((s0 + i) * each >= steps.count || e[i].x == -__builtin_inff()) continue;
             const float f = __builtin_amdgcn_exp2f(e[i].x - top);
             const float w[8] = {u[i][0].x, u[i][0].y, u[i][0].z, u[i][0].w, u[i][1].x, u[i][1].y, u[i][1].z, u[i][1].w};
             total += f * e[i].y;
@@ -1210,12 +1234,23 @@ static long long most_steps(const AttnArgs& a, int M, int S)
     return most < 1 ? 1 : most;
 }
 
-static void set_parts(AttnArgs& a, long long most, long long want, int unit)
+// Sets a tile's parts: `fill` of them, and by length, in parts of `longest`
+// steps, as far as they take no more than `blocks` workgroups (a thousand that
+// find nothing to do cost about 1 us) and 1 GB of workspace.
+static void set_parts(AttnArgs& a, int d, long long most, long long fill, long long longest, long long blocks)
 {
-    if (want < 1) want = 1;
-    if (want > 256) want = 256;
-    a.part = (int)(((most + want - 1) / want + unit - 1) / unit * unit);
-    a.splits = (int)((most + a.part - 1) / a.part);
+    if (fill > (most + 3) / 4) fill = (most + 3) / 4;
+    if (fill > 256) fill = 256;
+    if (fill < 1) fill = 1;
+    const long long room = a.lines ? (1ll << 30) / ((long long)a.lines * (d + 2) * 4) : 1;
+    long long more = (most + longest - 1) / longest;
+    if (more > 256) more = 256;
+    if (a.tiles && more > blocks / a.tiles) more = blocks / a.tiles;
+    if (more > room) more = room;
+    a.fill = (int)fill;
+    a.fill_inv = 1.0f / (float)fill;
+    a.longest = (int)longest;
+    a.splits = (int)(more > fill ? more : fill);
 }
 
 // The tiles of sixteen rows, for requests of at most `few` (token, head) rows.
@@ -1227,17 +1262,11 @@ static void shape16(AttnArgs& a, int d)
     const long long by_token = (long long)a.max_tokens * a.hq;
     a.by_tile = tiles * 16 < by_token;
     a.lines = (size_t)(a.by_tile ? tiles * 16 : by_token);
-    long long want = tiles > 0 ? (1024 + tiles - 1) / tiles : 1;
-    if (want > (most + 3) / 4) want = (most + 3) / 4;  // a step for each wavefront
     // With workgroups enough, parts of 1024 positions even out ragged lengths
     // (64 requests of up to 8000, 8 kv heads of 128, parts of 512, 1024, 2048
     // and 4096: 209, 204, 206 and 215 us; 40 of up to 3900, 36 kv heads, Q8:
-    // 111, 106, 108 and 113), within 1 GB of workspace.
-    long long by_len = (most + 31) / 32;
-    const long long room = a.lines ? (1ll << 30) / ((long long)a.lines * (d + 2) * 4) : 1;
-    if (by_len > room) by_len = room;
-    if (want < by_len && tiles < 65536) want = by_len;
-    set_parts(a, most, want, 4);
+    // 111, 106, 108 and 113).
+    set_parts(a, d, most, tiles > 0 ? (1024 + tiles - 1) / tiles : 1, 32, 8192);
 }
 
 // The tiles of 128 rows, for the others.
@@ -1248,16 +1277,15 @@ static void shape_rows(AttnArgs& a, int d)
     a.tiles = tile_slots(a.max_tokens, a.n_req, a.group, kRowsM) * a.hkv;
     a.by_tile = false;
     a.lines = (size_t)a.max_tokens * a.hq;
-    long long want = (512 + tiles - 1) / tiles;
-    if (want > (most + 3) / 4) want = (most + 3) / 4;
     // Where all tiles run at once the longest sets the time: parts of 1024
     // positions (520 tiles, 4 chunks over up to 2500 positions, heads of 128:
     // 91 to 88 us, Q8 234 to 197; 256 tiles over 5000: 85 to 73).  Where they
     // take turns, parts only add their sums' traffic (1850 tiles: 185 to 228).
     // Under a window all are of a length.
-    const long long by_len = (most * S + 1023) / 1024;
-    if (!a.window && tiles < 768 && want < by_len) want = by_len;
-    set_parts(a, most, want, 1);
+    const bool by_len = !a.window && tiles < 768;
+    // two workgroups a compute unit, and a quarter more, for some of the tile
+    // numbers hold no rows
+    set_parts(a, d, most, 640 / tiles, by_len ? 1024 / S : most, 4096);
 }
 
 // Rows of a request up to which the sixteen-row tiles take it.  Over 3000
