@@ -89,10 +89,10 @@ struct Steps {
 
 // Steps of a part, a multiple of UNIT, of a tile of `count` (at least 1): as
 // many parts as the chip has room for, though of no less than four steps, and
-// where those are long, parts of `longest` with a shorter last one (which
-// evens out better than parts alike).  By the steps that there are, not by the
-// bound that sizes the launch: with a bound 64 times the lengths that left one
-// part to each (64 requests of up to 2000: 130 us for 65).
+// where those are long, parts of `longest` with a shorter last one.  By the
+// steps that there are, not by the bound that sizes the launch: parts of a
+// bound 64 times the lengths left one part to each, among workgroups with
+// nothing to do (64 requests of up to 2000 positions: 130 us, now 65).
 template <int UNIT>
 __device__ __forceinline__ int steps_of_part(const AttnArgs& a, int count)
 {
@@ -241,9 +241,9 @@ __device__ __forceinline__ f32x4 mfma16(half8 a, half8 b, f32x4 c)
 // both enter as two fp16 halves (of the products of two low halves nothing is
 // left), so the sums are as good as fp32 ones.  These tiles wait for memory,
 // not for the matrix cores: one token each of 64 requests of up to 8000
-// positions, 32 heads over 8 kv heads of 128, fp16, 1.1 GB: 204 us, 5.4 TB/s
+// positions, 32 heads over 8 kv heads of 128, fp16, 1.1 GB: 205 us, 5.4 TB/s
 // (a large copy reaches 4.8); of 40 requests of up to 3900, 36 kv heads of
-// 64, Q8, 413 MB: 106 us, 3.9 TB/s (turning the codes to fp16 fills the issue
+// 64, Q8, 413 MB: 104 us, 4.0 TB/s (turning the codes to fp16 fills the issue
 // slots as well).  One request of 700 positions: 8 us, two launches and the
 // latency of page lookup, K, V and the join.
 
@@ -620,8 +620,8 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 3) void k_paged_attn16(AttnArgs 
 // one every 7 cycles, four on a SIMD one every 3; per step of 64 positions
 // and 32 rows 32 exponentials, as many conversions and 64 scalings and maxima
 // stand against 16 matrix instructions of 33 cycles): 4 chunks of 500 rows
-// over up to 2000 positions, 32 heads over 4 kv heads of 64, 22 GFLOP: 60 us,
-// 370 TFLOP/s; two of 1000 rows under a window of 1024, 8 kv heads of 128, 35
+// over up to 2000 positions, 32 heads over 4 kv heads of 64, 22 GFLOP: 59 us,
+// 375 TFLOP/s; two of 1000 rows under a window of 1024, 8 kv heads of 128, 35
 // GFLOP: 87 us, 400 TFLOP/s.  Sixteen-row tiles took 139 and 248.
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));

@@ -147,3 +147,54 @@ def test_steps(gpu, kind, window, sink):
         held = sum(P.up(len(h), PAGE) for h in history)
         assert sv.seq_len.tolist() == [len(h) for h in history] and sv.state[0].item() == PAGES - held
     assert done == [78, 8, 4]  # 37 + 40 + 1, 5 + 1 + 1 + 1 and 1 + 1 + 1 + 1 rows
+
+
+@pytest.mark.parametrize("kind", ["f16", "q8"])
+def test_a_captured_step_replayed_with_other_lengths(gpu, kind):
+    """One graph for every step, under bounds that hold them all: single tokens, chunks on both kinds of tiles, a step
+    that does not fit, requests that end."""
+    L = gpu.lib()
+    g = torch.Generator().manual_seed(22)
+    sv = Server(gpu, kind, 4, 96)
+    cache = Cache(kind, PAGES, PAGE, HKV, D, fill=float("nan"))
+    work = workspace(sv, cache, HQ, 0, 0)
+    q, k, v = (Rows("f32", 96, n) for n in (HQ * D, HKV * D, HKV * D))
+    qr, att = Rows(kind, 96, HQ * D), Rows(kind, 96, HQ * D, fill=0x3C)
+    graph = torch.cuda.CUDAGraph()
+    sync()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        on = P.stream(torch.cuda.current_stream())
+        gpu.check(L.nc_paged_plan(sv.pool_ref, sv.ref, on), "plan")
+        gpu.check(L.nc_paged_append(q.ref, k.ref, v.ref, qr.ref, cache.ref, sv.ref, None, 0, 0, on), "append")
+        gpu.check(L.nc_paged_attn(qr.ref, cache.ref, sv.ref, att.ref, HQ, 0, 0, P.ptr(work[0]), work[1], on), "attn")
+        gpu.check(L.nc_paged_commit(sv.pool_ref, sv.ref, P.ptr(sv.finished), on), "commit")
+    past, fitted = [0] * 4, []
+    for new, finished in (([40, 1, 0, 9], []), ([1, 1, 1, 1], []), ([40, 40, 3, 1], []), ([0, 41, 0, 0], []),
+                          ([20, 30, 40, 6], []), ([1, 1, 1, 1], [1]), ([1, 40, 1, 40], []), ([0, 0, 0, 0], [0, 3]),
+                          ([30, 0, 30, 2], []), ([1, 1, 1, 1], [])):
+        sv.new_len.copy_(ints(new))
+        sv.finished.copy_(ints([int(r in finished) for r in range(4)]))
+        for rows in (q, k, v):
+            rows.buf.view(torch.float32).copy_(torch.randn(96, rows.cols, generator=g))
+        before = att.buf.clone()
+        sync()
+        table = sv.table.tolist()  # requests that end here do so in steps that take no new page of theirs
+        graph.replay()
+        sync()
+        status = sv.state[2].item()
+        fitted.append(status == 0)
+        if status:
+            assert torch.equal(att.buf, before) and sv.seq_len.tolist() == past
+            continue
+        sv.facts(new, past)
+        after = sv.table.tolist()
+        assert all(after[r] == [-1] * sv.max_pages for r in finished)
+        tables = [table[r] if r in finished else after[r] for r in range(4)]
+        sv.past_slots = lambda r: [tables[r][i // PAGE] * PAGE + i % PAGE for i in range(past[r] + new[r])]
+        if sv.tokens:
+            want, tol = plain_attention(sv, cache, qr, HQ)
+            within(att.values()[:sv.tokens], want, rounded(kind, want, tol), f"{new} after {past}")
+        assert torch.equal(att.buf[sv.tokens:], before[sv.tokens:])
+        past = [0 if r in finished else p + n for r, (p, n) in enumerate(zip(past, new))]
+        assert sv.seq_len.tolist() == past
+    assert fitted == [True, True, True, False, True, True, True, True, True, True]
