@@ -39,7 +39,7 @@ struct LoraArgs {
 // shared memory, sixteen bytes at a time, pieces exchanged within rows by the
 // row's number so that neither side meets in a bank.  No barrier: a
 // wavefront's accesses to it keep their order.
-__device__ __forceinline__ int place16(int row, int piece) { return (row * 16 + (piece ^ row)) * 16; }  // of 256 B rows
+__device__ __forceinline__ int place16(int row, int piece) { return (row * 16 + (piece ^ row)) * 16; }  // 256 B rows
 __device__ __forceinline__ int place8(int row, int piece) { return (row * 8 + (piece ^ (row >> 1 & 7))) * 16; }  // 128 B
 
 // Piece of a row of RT * 32 bytes.

@@ -23,10 +23,11 @@
 // once (2^-11 each, as an fp16 result), since second halves of those would take
 // half as many matrix instructions again.  Over a Q8 cache these tiles do keep
 // them, for 131 instead of 100 us (4 chunks of 500 rows over up to 2000
-// positions, 32 heads over 4 of 64): its result rows may be Q8, whose codes turn with an
-// error far below their step (relative error of such rows 2.6e-3 with one
-// rounding each, 2.2e-4 without).  Probabilities are scaled by 2^14, so that what falls under
-// fp16's smallest number is below 2^-38 of the maximum's weight.
+// positions, 32 heads over 4 of 64): its result rows may be Q8, whose codes
+// turn with an error far below their step (relative error of such rows 2.6e-3
+// with one rounding each, 2.2e-4 without).  Probabilities are scaled by 2^14,
+// so that what falls under fp16's smallest number is below 2^-38 of the
+// maximum's weight.
 #include "nc_act.h"
 #include "nc_paged.h"
 
@@ -601,9 +602,9 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 3) void k_paged_attn16(AttnArgs 
 // ---- 128 rows a tile -----------------------------------------------------------
 //
 // One workgroup of four wavefronts per (tile, kv head, part of the
-// positions), 32 rows a wavefront, over steps of 64 (d = 128: 32) positions whose K and V
-// all four read from shared memory: each value comes from memory once per 128
-// rows.  The step after the one at work is already on its way to registers,
+// positions), 32 rows a wavefront, over steps of 64 (d = 128: 32) positions
+// whose K and V all four read from shared memory: each value comes from memory
+// once per 128 rows.  The step after the one at work is already on its way to registers,
 // and goes to the other of two buffers while the step is at work: one barrier
 // a step.  V is turned into V^T on its way (a thread turns four positions by
 // four values), its positions in the order in which a lane's probabilities
